@@ -95,6 +95,17 @@ SIGNATURES = {
     "dragon_hip_softmax_cross_entropy_loss_backward": (_int, [_int, _int, _i64, _i64, _i64, _i64,
                                                               _int, _vp, _vp, _vp, _vp, _vp, _sz,
                                                               _vp]),
+    "dragon_hip_rms_norm": (_int, [_int, _i64, _i64, _f32] + [_vp] * 7),
+    "dragon_hip_rms_norm_quant": (_int, [_int, _i64, _i64, _i64, _f32] + [_vp] * 8),
+    "dragon_hip_rms_norm_grad_scratch_bytes": (_sz, [_int, _i64, _i64]),
+    "dragon_hip_rms_norm_grad": (_int, [_int, _i64, _i64] + [_vp] * 8 + [_sz, _vp]),
+    "dragon_hip_topk_distillation_loss_scratch_bytes": (_sz, [_int, _i64, _i64]),
+    "dragon_hip_topk_distillation_loss_forward": (_int, [_int, _int, _i64, _i64, _i64, _f32, _f32] +
+                                                  [_vp] * 6 + [_sz, _vp]),
+    "dragon_hip_topk_distillation_loss_backward": (_int, [_int, _int, _i64, _i64, _i64, _f32, _f32] +
+                                                   [_vp] * 7),
+    "dragon_hip_draft_verify_scratch_bytes": (_sz, [_int, _i64, _i64, _i64]),
+    "dragon_hip_draft_verify": (_int, [_int, _int, _i64, _i64, _i64] + [_vp] * 9 + [_sz, _vp]),
     "dragon_hip_group_norm_forward_scratch_bytes": (_sz, [_int, _i64, _i64, _i64, _i64, _int]),
     "dragon_hip_group_norm_forward": (_int, [_int, _i64, _i64, _i64, _i64, _int, _f32, _vp, _vp,
                                              _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

@@ -93,6 +93,26 @@ extern "C" int dragon_hip_plan_name(const char* op, int dtype, int layout, const
       rc = dragon_hip_softmax_cross_entropy_loss_backward(dtype, DRAGON_HIP_I64, dim(0), dim(1),
                                                           dim(2), 255, 4 /* VALID */, fake(0),
                                                           fake(1), fake(2), fake(3), fake(4), big, s);
+    } else if (!strcmp(op, "rms_norm")) {
+      rc = dragon_hip_rms_norm(dtype, dim(0), dim(1), 1e-5f, fake(0), fake(1), fake(2), fake(3), fake(4),
+                               fake(5), s);
+    } else if (!strcmp(op, "rms_norm_quant")) {
+      rc = dragon_hip_rms_norm_quant(dtype, dim(0), dim(1), dim(2), 1e-5f, fake(0), fake(1), fake(2),
+                                     fake(3), fake(4), fake(5), fake(6), s);
+    } else if (!strcmp(op, "rms_norm_grad")) {
+      rc = dragon_hip_rms_norm_grad(dtype, dim(0), dim(1), fake(0), fake(1), fake(2), fake(3), fake(4),
+                                    fake(5), fake(6), fake(7), big, s);
+    } else if (!strcmp(op, "topk_distillation_loss_forward")) {
+      rc = dragon_hip_topk_distillation_loss_forward(dtype, DRAGON_HIP_I64, dim(0), dim(1), dim(2), 1.f,
+                                                     -1.f, fake(0), fake(1), fake(2), fake(3), fake(4),
+                                                     fake(5), big, s);
+    } else if (!strcmp(op, "topk_distillation_loss_backward")) {
+      rc = dragon_hip_topk_distillation_loss_backward(dtype, DRAGON_HIP_I64, dim(0), dim(1), dim(2), 1.f,
+                                                      -1.f, fake(0), fake(1), fake(2), fake(3), fake(4),
+                                                      fake(5), s);
+    } else if (!strcmp(op, "draft_verify")) {
+      rc = dragon_hip_draft_verify(dtype, DRAGON_HIP_I64, dim(0), dim(1), dim(2), fake(0), fake(1),
+                                   fake(2), fake(3), fake(4), fake(5), fake(6), fake(7), fake(8), big, s);
     } else {
       known = false;
     }

@@ -356,6 +356,84 @@ DEFINE_SPARSE_LOSS_LAUNCHERS(double, int);
 DEFINE_SPARSE_LOSS_LAUNCHERS(double, int64_t);
 #undef DEFINE_SPARSE_LOSS_LAUNCHERS
 
+#define DEFINE_RMS_NORM_LAUNCHERS(T, AccT)                                                        \
+  template <>                                                                                     \
+  void RMSNorm<T, AccT, HIPContext>(const int N, const int C, const float epsilon, const T* x,    \
+                                    const T* residual, const AccT* gamma, T* h, AccT* rsig, T* y, \
+                                    HIPContext* ctx) {                                            \
+    HIP_CHECK(dragon_hip_rms_norm(Tag<T>(), N, C, epsilon, x, residual, gamma, h, rsig, y,        \
+                                  ctx->hip_stream()));                                            \
+  }                                                                                               \
+  template <>                                                                                     \
+  void RMSNormGrad<T, AccT, HIPContext>(const int N, const int C, const T* h, const AccT* rsig,   \
+                                        const AccT* gamma, const T* dy, const T* dh,              \
+                                        AccT* dgamma, T* dx, HIPContext* ctx) {                   \
+    const size_t bytes = dragon_hip_rms_norm_grad_scratch_bytes(Tag<T>(), N, C);                  \
+    HIP_CHECK(dragon_hip_rms_norm_grad(Tag<T>(), N, C, h, rsig, gamma, dy, dh, dgamma, dx,        \
+                                       Scratch(ctx, bytes), bytes, ctx->hip_stream()));           \
+  }
+
+DEFINE_RMS_NORM_LAUNCHERS(float16, float);
+DEFINE_RMS_NORM_LAUNCHERS(bfloat16, float);
+DEFINE_RMS_NORM_LAUNCHERS(float, float);
+DEFINE_RMS_NORM_LAUNCHERS(double, double);
+#undef DEFINE_RMS_NORM_LAUNCHERS
+
+#define DEFINE_RMS_NORM_QUANT_LAUNCHER(T)                                                         \
+  template <>                                                                                     \
+  void RMSNormQuant<T, HIPContext>(const int N, const int C, const int group, const float epsilon, \
+                                   const T* x, const T* residual, const float* gamma, T* h,       \
+                                   float* rsig, uint8_t* q, float* scale, HIPContext* ctx) {      \
+    HIP_CHECK(dragon_hip_rms_norm_quant(Tag<T>(), N, C, group, epsilon, x, residual, gamma, h,    \
+                                        rsig, q, scale, ctx->hip_stream()));                      \
+  }
+
+DEFINE_RMS_NORM_QUANT_LAUNCHER(float16);
+DEFINE_RMS_NORM_QUANT_LAUNCHER(bfloat16);
+DEFINE_RMS_NORM_QUANT_LAUNCHER(float);
+#undef DEFINE_RMS_NORM_QUANT_LAUNCHER
+
+#define DEFINE_TOKEN_LAUNCHERS(T, AccT, IndexT)                                                   \
+  template <>                                                                                     \
+  void TopKDistillationLossForward<T, AccT, IndexT, HIPContext>(                                  \
+      const int N, const int C, const int K, const float temperature, const float normalizer,     \
+      const T* x, const IndexT* index, const AccT* teacher, AccT* stats, AccT* loss,              \
+      HIPContext* ctx) {                                                                          \
+    const size_t bytes = dragon_hip_topk_distillation_loss_scratch_bytes(Tag<T>(), N, C);         \
+    HIP_CHECK(dragon_hip_topk_distillation_loss_forward(                                          \
+        Tag<T>(), TargetTag<IndexT>(), N, C, K, temperature, normalizer, x, index, teacher,       \
+        stats, loss, Scratch(ctx, bytes), bytes, ctx->hip_stream()));                             \
+  }                                                                                               \
+  template <>                                                                                     \
+  void TopKDistillationLossBackward<T, AccT, IndexT, HIPContext>(                                 \
+      const int N, const int C, const int K, const float temperature, const float normalizer,     \
+      const T* x, const IndexT* index, const AccT* teacher, const AccT* stats, const AccT* dl,    \
+      T* dx, HIPContext* ctx) {                                                                   \
+    HIP_CHECK(dragon_hip_topk_distillation_loss_backward(                                         \
+        Tag<T>(), TargetTag<IndexT>(), N, C, K, temperature, normalizer, x, index, teacher,       \
+        stats, dl, dx, ctx->hip_stream()));                                                       \
+  }                                                                                               \
+  template <>                                                                                     \
+  void DraftVerify<T, IndexT, HIPContext>(                                                        \
+      const int B, const int K, const int C, const T* target, const T* draft,                     \
+      const IndexT* drafted, const IndexT* lengths, const float* u_accept, const float* u_sample, \
+      IndexT* tokens, IndexT* accepted, HIPContext* ctx) {                                        \
+    const size_t bytes = dragon_hip_draft_verify_scratch_bytes(Tag<T>(), B, K, C);                \
+    HIP_CHECK(dragon_hip_draft_verify(Tag<T>(), TargetTag<IndexT>(), B, K, C, target, draft,      \
+                                      drafted, lengths, u_accept, u_sample, tokens, accepted,     \
+                                      Scratch(ctx, bytes), bytes, ctx->hip_stream()));            \
+  }
+
+DEFINE_TOKEN_LAUNCHERS(float16, float, int);
+DEFINE_TOKEN_LAUNCHERS(float16, float, int64_t);
+DEFINE_TOKEN_LAUNCHERS(bfloat16, float, int);
+DEFINE_TOKEN_LAUNCHERS(bfloat16, float, int64_t);
+DEFINE_TOKEN_LAUNCHERS(float, float, int);
+DEFINE_TOKEN_LAUNCHERS(float, float, int64_t);
+DEFINE_TOKEN_LAUNCHERS(double, double, int);
+DEFINE_TOKEN_LAUNCHERS(double, double, int64_t);
+#undef DEFINE_TOKEN_LAUNCHERS
+
 } // namespace kernels
 
 namespace math {

@@ -147,6 +147,37 @@ void ReduceLossGrad(const int N, const int num_masks, const float normalizer, co
 template <typename T, class Context>
 void BroadcastLossGrad(const int N, const int S, const int C, const T* dl, T* dx, Context* ctx);
 
+// Operators of language models (no counterpart in the reference; semantics in dragon_hip.h).
+template <typename T, typename AccT, class Context>
+void RMSNorm(const int N, const int C, const float epsilon, const T* x, const T* residual,
+             const AccT* gamma, T* h, AccT* rsig, T* y, Context* ctx);
+
+template <typename T, class Context>
+void RMSNormQuant(const int N, const int C, const int group, const float epsilon, const T* x,
+                  const T* residual, const float* gamma, T* h, float* rsig, uint8_t* q, float* scale,
+                  Context* ctx);
+
+template <typename T, typename AccT, class Context>
+void RMSNormGrad(const int N, const int C, const T* h, const AccT* rsig, const AccT* gamma,
+                 const T* dy, const T* dh, AccT* dgamma, T* dx, Context* ctx);
+
+// normalizer: 0 for a loss per row, -1 for the rows that count, else the divisor.
+template <typename T, typename AccT, typename IndexT, class Context>
+void TopKDistillationLossForward(const int N, const int C, const int K, const float temperature,
+                                 const float normalizer, const T* x, const IndexT* index,
+                                 const AccT* teacher, AccT* stats, AccT* loss, Context* ctx);
+
+template <typename T, typename AccT, typename IndexT, class Context>
+void TopKDistillationLossBackward(const int N, const int C, const int K, const float temperature,
+                                  const float normalizer, const T* x, const IndexT* index,
+                                  const AccT* teacher, const AccT* stats, const AccT* dl, T* dx,
+                                  Context* ctx);
+
+template <typename T, typename IndexT, class Context>
+void DraftVerify(const int B, const int K, const int C, const T* target, const T* draft,
+                 const IndexT* drafted, const IndexT* lengths, const float* u_accept,
+                 const float* u_sample, IndexT* tokens, IndexT* accepted, Context* ctx);
+
 // Fused operator bodies (see the header comment).
 template <typename T, typename AccT, class Context>
 void GroupNormForward(const int N, const int G, const int D, const int S, const string& data_format,

@@ -1,0 +1,116 @@
+#include "operators/rms_norm_op.h"
+
+#include <climits>
+
+#include "core/gradient.h"
+#include "kernels/op_kernels.h"
+
+namespace dragon {
+
+template <class Context>
+template <typename T>
+void RMSNormOp<Context>::DoRunWithType() {
+  using AccT = typename math::Traits<T>::accumulator_type;
+  Tensor& X = Input(0);
+  Tensor& W = Input(1);
+  GET_OP_AXIS_ARG(axis, X.ndim(), -1);
+  const int64_t rows = X.count(0, axis), width = X.count(axis);
+  INITIALIZE_TENSOR_VIA_SPEC(W, vec64_t({width}), AccT);
+  CHECK_EQ(OutputSize(), InputSize() - 1) << "\nA residual's sum is the second output.";
+  const T* residual = nullptr;
+  T* h = nullptr;
+  if (InputSize() > 2) {
+    INITIALIZE_TENSOR_VIA_SPEC(Input(2), X.dims(), T);
+    residual = Input(2).template data<T, Context>(ctx());
+    h = Output(1)->ReshapeLike(X)->template mutable_data<T, Context>(ctx());
+  }
+  kernels::RMSNorm(static_cast<int>(rows), static_cast<int>(width), static_cast<float>(epsilon_),
+                   X.template data<T, Context>(ctx()), residual, W.template data<AccT, Context>(ctx()), h,
+                   Output("X_rsig")->Reshape({rows})->template mutable_data<AccT, Context>(ctx()),
+                   Output(0)->ReshapeLike(X)->template mutable_data<T, Context>(ctx()), ctx());
+}
+
+template <class Context>
+template <typename T>
+void RMSNormGradientOp<Context>::DoRunWithType() {
+  using AccT = typename math::Traits<T>::accumulator_type;
+  Tensor& H = Input(0);
+  Tensor& W = Input(1);
+  GET_OP_AXIS_ARG(axis, H.ndim(), -1);
+  const int64_t rows = H.count(0, axis), width = H.count(axis);
+  INITIALIZE_TENSOR_VIA_SPEC(W, vec64_t({width}), AccT);
+  INITIALIZE_TENSOR_VIA_SPEC(Input(2), H.dims(), T);
+  const T* dh = nullptr;
+  if (InputSize() > 3) {
+    INITIALIZE_TENSOR_VIA_SPEC(Input(3), H.dims(), T);
+    dh = Input(3).template data<T, Context>(ctx());
+  }
+  T* dx = Output(0)->ReshapeLike(H)->template mutable_data<T, Context>(ctx());
+  kernels::RMSNormGrad(static_cast<int>(rows), static_cast<int>(width),
+                       H.template data<T, Context>(ctx()),
+                       Input("X_rsig").template data<AccT, Context>(ctx()),
+                       W.template data<AccT, Context>(ctx()), Input(2).template data<T, Context>(ctx()), dh,
+                       Output(1)->ReshapeLike(W)->template mutable_data<AccT, Context>(ctx()), dx, ctx());
+  if (OutputSize() > 2) {  // X and the residual are summed: one gradient for both, in a tensor each
+    CHECK_LE(H.count(), static_cast<int64_t>(INT_MAX)) << "\nToo many elements for a copied gradient.";
+    math::Copy(static_cast<int>(H.count()), static_cast<const T*>(dx),
+               Output(2)->ReshapeLike(H)->template mutable_data<T, Context>(ctx()), ctx());
+  }
+}
+
+template <class Context>
+template <typename T>
+void RMSNormQuantOp<Context>::DoRunWithType() {
+  Tensor& X = Input(0);
+  Tensor& W = Input(1);
+  GET_OP_AXIS_ARG(axis, X.ndim(), -1);
+  const int64_t rows = X.count(0, axis), width = X.count(axis);
+  INITIALIZE_TENSOR_VIA_SPEC(W, vec64_t({width}), float);
+  CHECK_EQ(OutputSize(), InputSize()) << "\nA residual's sum is the third output.";
+  CHECK_GE(group_size_, 0) << "\nExcepted a <group_size> of 0, 32, 64, 128 or 256.";
+  const T* residual = nullptr;
+  T* h = nullptr;
+  if (InputSize() > 2) {
+    INITIALIZE_TENSOR_VIA_SPEC(Input(2), X.dims(), T);
+    residual = Input(2).template data<T, Context>(ctx());
+    h = Output(2)->ReshapeLike(X)->template mutable_data<T, Context>(ctx());
+  }
+  vec64_t scale_dims(X.dims().begin(), X.dims().begin() + axis);
+  scale_dims.push_back(group_size_ > 0 ? (width + group_size_ - 1) / group_size_ : 1);
+  kernels::RMSNormQuant(
+      static_cast<int>(rows), static_cast<int>(width), static_cast<int>(group_size_),
+      static_cast<float>(epsilon_), X.template data<T, Context>(ctx()), residual,
+      W.template data<float, Context>(ctx()), h, static_cast<float*>(nullptr),
+      Output(0)->ReshapeLike(X)->template mutable_data<uint8_t, Context>(ctx()),
+      Output(1)->Reshape(scale_dims)->template mutable_data<float, Context>(ctx()), ctx());
+}
+
+DEPLOY_HIP_OPERATOR(RMSNorm);
+DEPLOY_HIP_OPERATOR(RMSNormGradient);
+DEPLOY_HIP_OPERATOR(RMSNormQuant);
+
+OPERATOR_SCHEMA(RMSNorm).NumInputs(2, 3).NumOutputs(1, 2);          // X, W[, R] -> Y[, H]
+OPERATOR_SCHEMA(RMSNormGradient).NumInputs(3, 4).NumOutputs(2, 3);  // H, W, dY[, dH] -> dX, dW[, dR]
+OPERATOR_SCHEMA(RMSNormQuant).NumInputs(2, 3).NumOutputs(2, 3);     // X, W[, R] -> Q, S[, H]
+
+namespace {
+
+class RMSNormGradientMaker final : public GradientMakerBase {
+ public:
+  using GradientMakerBase::GradientMakerBase;
+  void CreateGradientDefs() override {
+    if (def().input.size() < 3) {
+      AddGradientDef("RMSNormGradient", {I(0), I(1), GO(0)}, {GI(0), GI(1)});
+      return;
+    }
+    vector<string> inputs = {O(1), I(1), GO(0)};
+    if (!GO(1).empty() && GO(1) != "NULL") inputs.push_back(GO(1));
+    AddGradientDef("RMSNormGradient", inputs, {GI(0), GI(1), GI(2)});
+  }
+};
+
+} // namespace
+
+REGISTER_GRADIENT(RMSNorm, RMSNormGradientMaker);
+
+} // namespace dragon

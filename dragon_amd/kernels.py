@@ -302,6 +302,132 @@ def broadcast_loss_grad(N, S, C, dl, dx):
     _call("dragon_hip_broadcast_loss_grad", dtype_tag(dx), N, S, C, _ptr(dl), _ptr(dx), _stream())
 
 
+# ---------------------------------------------------------------- operators of language models
+
+_BYTE_DTYPES = (torch.uint8, torch.float8_e4m3fn)
+_ACC_DTYPES = {0: torch.float32, 1: torch.float32, 2: torch.float32, 3: torch.float64}
+
+
+class _Args:
+    """Checks the tensors of one call against its sizes and gives their addresses: all on the
+    current device, contiguous, of the type asked for and of at least so many elements."""
+
+    def __init__(self):
+        self.device = torch.cuda.current_device()
+
+    def __call__(self, t, numel, dtype, optional=False):
+        if t is None:
+            if optional or numel == 0:
+                return None
+            raise ValueError("a tensor is missing")
+        if t.get_device() != self.device:
+            raise ValueError("kernel arguments must live in the memory of the current device")
+        if not t.is_contiguous():
+            raise ValueError("kernel arguments must be contiguous")
+        if t.dtype is not dtype and not (type(dtype) is tuple and t.dtype in dtype):
+            raise TypeError("a tensor of %s where %s is expected" % (t.dtype, dtype))
+        if t.numel() < numel:
+            raise ValueError("a tensor of %d elements where the sizes ask for %d" % (t.numel(), numel))
+        return t.data_ptr()
+
+    def stream(self):
+        return torch._C._cuda_getCurrentRawStream(self.device)
+
+    def scratch(self, nbytes):
+        """Scratch for the current stream. While a graph is being captured it comes from that
+        graph's own memory, so that graphs share none and a later, larger call cannot free it."""
+        if nbytes == 0:
+            return None
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return workspace(nbytes, torch.device("cuda", self.device))
+
+
+def _sizes(*sizes):
+    if min(sizes) < 0:
+        raise ValueError("negative size in %s" % (sizes,))
+
+
+def rms_norm(N, C, epsilon, x, residual, gamma, h, rsig, y):
+    """h = x + residual, y = h / sqrt(mean(h^2) + epsilon) * gamma over rows of C. residual, h and
+    rsig may be None; y and h may be the tensors x or residual themselves."""
+    _sizes(N, C)
+    a, tag, n = _Args(), dtype_tag(x), N * C
+    acc, dt = _ACC_DTYPES[tag], x.dtype
+    _call("dragon_hip_rms_norm", tag, N, C, epsilon, a(x, n, dt), a(residual, n, dt, True),
+          a(gamma, C, acc), a(h, n, dt, True), a(rsig, N, acc, True), a(y, n, dt), a.stream())
+
+
+def rms_norm_quant(N, C, group, epsilon, x, residual, gamma, h, rsig, q, scale):
+    """rms_norm with y as e4m3 codes (uint8 or float8_e4m3fn) and a float32 scale per group of
+    columns (32, 64, 128 or 256; 0: per row): y = q * scale."""
+    _sizes(N, C, group)
+    a, tag, n = _Args(), dtype_tag(x), N * C
+    dt, groups = x.dtype, -(-C // group) if group else 1
+    _call("dragon_hip_rms_norm_quant", tag, N, C, group, epsilon, a(x, n, dt), a(residual, n, dt, True),
+          a(gamma, C, _ACC_DTYPES[tag]), a(h, n, dt, True), a(rsig, N, _ACC_DTYPES[tag], True),
+          a(q, n, _BYTE_DTYPES), a(scale, N * groups, torch.float32), a.stream())
+
+
+def rms_norm_grad(N, C, h, rsig, gamma, dy, dh, dgamma, dx):
+    """Gradient of rms_norm from its h (x where there was no residual) and rsig; dh, the gradient
+    that arrives through h, may be None. dx may be the tensor dy or dh itself."""
+    _sizes(N, C)
+    a, tag, n = _Args(), dtype_tag(h), N * C
+    acc, dt = _ACC_DTYPES[tag], h.dtype
+    need = _lib.lib().dragon_hip_rms_norm_grad_scratch_bytes(tag, N, C)
+    ws = a.scratch(need)
+    _call("dragon_hip_rms_norm_grad", tag, N, C, a(h, n, dt), a(rsig, N, acc), a(gamma, C, acc),
+          a(dy, n, dt), a(dh, n, dt, True), a(dgamma, C, acc), a(dx, n, dt),
+          None if ws is None else ws.data_ptr(), need, a.stream())
+
+
+def _normalizer(reduction, N):
+    """The divisor of a reduction over N rows: 0 for none, -1 for the rows that count."""
+    return {"NONE": 0.0, "SUM": 1.0, "MEAN": float(max(N, 1)), "BATCH_MEAN": float(max(N, 1)),
+            "VALID": -1.0}[reduction.upper()]
+
+
+def topk_distillation_loss_forward(N, C, K, temperature, reduction, x, index, teacher, stats, loss):
+    """Loss of the logits x [N, C] against a teacher's K top logits [N, K] of the classes index
+    [N, K]; entries outside [0, C) are not listed, rows that list nothing are ignored. stats
+    [N + 1] is for the backward call."""
+    _sizes(N, C, K)
+    a, tag = _Args(), dtype_tag(x)
+    acc, normalizer = _ACC_DTYPES[tag], _normalizer(reduction, N)
+    need = _lib.lib().dragon_hip_topk_distillation_loss_scratch_bytes(tag, N, C)
+    ws = a.scratch(need)
+    _call("dragon_hip_topk_distillation_loss_forward", tag, target_tag(index), N, C, K, temperature,
+          normalizer, a(x, N * C, x.dtype), a(index, N * K, index.dtype), a(teacher, N * K, acc),
+          a(stats, N + 1, acc), a(loss, 1 if normalizer else N, acc),
+          None if ws is None else ws.data_ptr(), need, a.stream())
+
+
+def topk_distillation_loss_backward(N, C, K, temperature, reduction, x, index, teacher, stats, dl, dx):
+    """Gradient with respect to x; dx may be the tensor x itself."""
+    _sizes(N, C, K)
+    a, tag = _Args(), dtype_tag(x)
+    acc, normalizer = _ACC_DTYPES[tag], _normalizer(reduction, N)
+    _call("dragon_hip_topk_distillation_loss_backward", tag, target_tag(index), N, C, K, temperature,
+          normalizer, a(x, N * C, x.dtype), a(index, N * K, index.dtype), a(teacher, N * K, acc),
+          a(stats, N + 1, acc), a(dl, 1 if normalizer else N, acc), a(dx, N * C, x.dtype), a.stream())
+
+
+def draft_verify(B, K, C, target, draft, drafted, lengths, u_accept, u_sample, tokens, accepted):
+    """Verifies drafted [B, K] against the probabilities target [B, K + 1, C] and draft [B, K, C]
+    (None: drafted without sampling): tokens [B, K + 1] = the accepted ones, one that is sampled
+    where they end, -1 behind it; accepted [B] = how many. lengths [B] may be None (K each)."""
+    _sizes(B, K, C)
+    a, tag = _Args(), dtype_tag(target)
+    dt, it = target.dtype, tokens.dtype
+    need = _lib.lib().dragon_hip_draft_verify_scratch_bytes(tag, B, K, C)
+    ws = a.scratch(need)
+    _call("dragon_hip_draft_verify", tag, target_tag(tokens), B, K, C, a(target, B * (K + 1) * C, dt),
+          a(draft, B * K * C, dt, True), a(drafted, B * K, it), a(lengths, B, it, True),
+          a(u_accept, B * K, torch.float32), a(u_sample, B, torch.float32), a(tokens, B * (K + 1), it),
+          a(accepted, B, it), None if ws is None else ws.data_ptr(), need, a.stream())
+
+
 # ---------------------------------------------------------------- fused operator bodies
 
 def softmax_cross_entropy_loss_forward(N, S, C, ignore_index, reduction, x, target, prob, loss):

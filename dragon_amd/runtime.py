@@ -297,6 +297,27 @@ def softmax_cross_entropy_loss(tape, inputs, axis=-1, ignore_index=None, reducti
                     reduction=reduction.upper())
 
 
+def rms_norm(tape, inputs, axis=-1, epsilon=1e-5):
+    """(x, weight) -> y, or (x, weight, residual) -> [y, h] with h = x + residual."""
+    return tape.run("RMSNorm", inputs, num_outputs=len(inputs) - 1, axis=axis, epsilon=float(epsilon))
+
+
+def rms_norm_quant(tape, inputs, axis=-1, epsilon=1e-5, group_size=0):
+    """(x, weight) -> [codes, scales], or (x, weight, residual) -> [codes, scales, h]; e4m3 codes as uint8."""
+    return tape.run("RMSNormQuant", inputs, num_outputs=len(inputs), axis=axis, epsilon=float(epsilon),
+                    group_size=int(group_size))
+
+
+def topk_distillation_loss(tape, inputs, temperature=1.0, reduction="valid"):
+    """(logits, classes, teacher's logits) -> loss."""
+    return tape.run("TopKDistillationLoss", inputs, temperature=float(temperature), reduction=reduction.upper())
+
+
+def draft_verify(tape, inputs):
+    """(target, drafted, lengths, u_accept, u_sample[, draft]) -> [tokens, accepted]."""
+    return tape.run("DraftVerify", inputs, num_outputs=2)
+
+
 def softmax(tape, inputs, axis=-1):
     return tape.run("Softmax", inputs, axis=axis)
 

@@ -2,7 +2,9 @@
  * dragon_hip.h - C ABI of the MI355X (gfx950) kernel library behind Dragon's
  * kernels:: / math:: interface for LayerNorm, GroupNorm, BatchNorm, Moments,
  * Softmax / LogSoftmax and their siblings on the same reduction skeleton
- * (L1/L2Norm, ReduceSum, softmax cross-entropy loss).
+ * (L1/L2Norm, ReduceSum, softmax cross-entropy loss), and of operators of
+ * language models on that skeleton (RMSNorm, distillation, verification of
+ * drafted tokens).
  *
  * Each entry point replaces one function template of the reference (cited as
  * file:line relative to the reference tree). A `kernels::X<T, AccT, HIPContext>`
@@ -44,7 +46,7 @@ typedef enum {
   DRAGON_HIP_BF16 = 1, /* dragon::bfloat16 (dragon/core/types.h:40-42) */
   DRAGON_HIP_F32 = 2,
   DRAGON_HIP_F64 = 3,
-  DRAGON_HIP_I32 = 4, /* class-index targets of the loss kernels only */
+  DRAGON_HIP_I32 = 4, /* class indices and tokens only */
   DRAGON_HIP_I64 = 5
 } dragon_hip_dtype;
 
@@ -341,6 +343,99 @@ int dragon_hip_softmax_cross_entropy_loss_backward(int dtype, int target_dtype, 
                                                    void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Operators of language models beside the families above. No counterpart in */
+/* the reference; conventions, dtypes and errors are those of this header.   */
+/* ------------------------------------------------------------------------ */
+
+/* RMSNorm of s = x + residual (residual may be NULL: s = x), per row of C:
+ *   rsig = 1 / sqrt(mean(s^2) + eps),  y = s * rsig * gamma,  h = s
+ * x, residual, y, h: T[N, C]; gamma: AccT[C]; rsig: AccT[N]. s is held in AccT
+ * and rounded once into h and once into y. h and rsig may be NULL where the
+ * caller has no use for them. Each output may be the very buffer of x or of
+ * residual (y and h may not be the same buffer). N and C below 2^31. */
+int dragon_hip_rms_norm(int dtype, int64_t N, int64_t C, float eps, const void* x,
+                        const void* residual, const void* gamma, void* h, void* rsig, void* y,
+                        void* stream);
+
+/* The same with y in 8 bits (OCP e4m3) and a scale per group of `group`
+ * consecutive columns of a row (32, 64, 128 or 256; 0: the whole row is one
+ * group; the last group of a row may be shorter):
+ *   scale = max(max|y|, 1e-30) / 448,  q = e4m3(y / scale)
+ * q: one byte per element [N, C]; scale: float[N, ceil(C / group)]. A NaN in y
+ * becomes a NaN code and is passed over by the maximum. dtype F16, BF16 or
+ * F32 (DRAGON_HIP_EDTYPE otherwise). */
+int dragon_hip_rms_norm_quant(int dtype, int64_t N, int64_t C, int64_t group, float eps,
+                              const void* x, const void* residual, const void* gamma, void* h,
+                              void* rsig, void* q, void* scale, void* stream);
+
+/* Gradient of dragon_hip_rms_norm, given its h (x itself where no residual was
+ * added) and rsig; dh (may be NULL) is the gradient that arrives through h:
+ *   z = dy * gamma,  dx = dh + rsig * (z - h * rsig^2 * mean(z * h)),
+ *   dgamma = sum over rows of dy * h * rsig
+ * dx is the gradient of x and of residual alike. dx may be the very buffer of
+ * dy or of dh. dgamma: AccT[C], overwritten (zero for N = 0). The sums have a
+ * fixed order: equal inputs give equal bits. */
+size_t dragon_hip_rms_norm_grad_scratch_bytes(int dtype, int64_t N, int64_t C);
+int dragon_hip_rms_norm_grad(int dtype, int64_t N, int64_t C, const void* h, const void* rsig,
+                             const void* gamma, const void* dy, const void* dh, void* dgamma,
+                             void* dx, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Distillation of a student x: T[N, C] (logits) from a teacher's top logits,
+ * index: I32 / I64 [N, K] (classes) and teacher: AccT[N, K] (logits), at a
+ * temperature t:
+ *   p = softmax over the K listed entries of teacher / t,  s = softmax(x / t)
+ *   loss of a row = t^2 * sum_k p_k (log p_k - log s[index_k])
+ *   dx = dl * t * (s - p scattered to its classes) / divisor
+ * An entry whose class is outside [0, C) or whose teacher logit is -inf is not
+ * listed; a class that is listed twice receives both shares. A row that lists
+ * nothing is ignored: its loss and gradient are 0 whatever its logits hold, and
+ * it is not read. A row whose logits are all -inf, or that holds NaN or +inf,
+ * has a NaN loss and NaN gradients.
+ * normalizer: 0 keeps a loss per row (loss: AccT[N], dl: AccT[N]); otherwise
+ * loss = sum of rows / max(divisor, 1) (AccT[1], dl: AccT[1], the gradient
+ * divides by max(divisor, 0.5), as ReduceLossGrad) with divisor = normalizer,
+ * or the number of rows that are not ignored where normalizer < 0.
+ * stats: AccT[N + 1], written by the forward for the backward call: log sum
+ * exp(x / t) of each row (+inf for an ignored one), then the divisor (1 for
+ * normalizer 0). dx may be the very buffer of x. 1 <= K <= 1024, t > 0, N and C
+ * below 2^31. The sums have a fixed order. */
+size_t dragon_hip_topk_distillation_loss_scratch_bytes(int dtype, int64_t N, int64_t C);
+int dragon_hip_topk_distillation_loss_forward(int dtype, int index_dtype, int64_t N, int64_t C,
+                                              int64_t K, float temperature, float normalizer,
+                                              const void* x, const void* index,
+                                              const void* teacher, void* stats, void* loss,
+                                              void* scratch, size_t scratch_bytes, void* stream);
+int dragon_hip_topk_distillation_loss_backward(int dtype, int index_dtype, int64_t N, int64_t C,
+                                               int64_t K, float temperature, float normalizer,
+                                               const void* x, const void* index,
+                                               const void* teacher, const void* stats,
+                                               const void* dl, void* dx, void* stream);
+
+/* Verification of drafted tokens, per sequence b of B:
+ *   target   T[B, K + 1, C]  the target's probabilities at each drafted position and
+ *                            at the one behind the last
+ *   draft    T[B, K, C]      the draft's probabilities, or NULL where tokens were drafted
+ *                            without sampling (all of the probability on the token)
+ *   drafted  I32 / I64 [B, K] drafted tokens;  lengths the same type [B], how many of the K
+ *                            are drafted (clamped to 0 .. K; NULL: all K)
+ *   u_accept float[B, K], u_sample float[B]: uniform random numbers of [0, 1)
+ * Position i is accepted while u_accept[i] * draft[i, d] < target[i, d], d = drafted[i]; the
+ * first refusal n ends it and one token is sampled from max(target[n] - draft[n], 0); where
+ * all are accepted, from target[n], n = lengths[b]. The sample is the lowest class whose
+ * running sum exceeds u_sample * total (u >= 1: the last class of non-zero weight). A
+ * residual without weight gives way to target[n], and no weight there to token -1.
+ * tokens (index type, [B, K + 1]) = the n accepted, the sampled one, -1 behind it;
+ * accepted (index type, [B]) = n. Probabilities that are negative or not finite count as 0; a
+ * drafted token outside [0, C) is refused. Comparisons and sums are held in 64 bits. K may be
+ * 0 (draft, drafted, u_accept unused). B, K and C below 2^31. */
+size_t dragon_hip_draft_verify_scratch_bytes(int dtype, int64_t B, int64_t K, int64_t C);
+int dragon_hip_draft_verify(int dtype, int index_dtype, int64_t B, int64_t K, int64_t C,
+                            const void* target, const void* draft, const void* drafted,
+                            const void* lengths, const void* u_accept, const void* u_sample,
+                            void* tokens, void* accepted, void* scratch, size_t scratch_bytes,
+                            void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Operator-level fused entry points: one call for a kernel sequence that a  */
 /* Dragon operator body issues back to back, so that x is read once where    */
 /* the chip can hold the reduction unit on-die. Results equal the sequence.  */
@@ -455,9 +550,12 @@ int dragon_hip_group_norm_grad_timeline(int dtype, int64_t N, int64_t G, int64_t
  * "group_norm_grad", "batch_norm_training_forward", "batch_norm_training_backward",
  * "softmax", "log_softmax", "softmax_grad", "log_softmax_grad", "l1_norm",
  * "l2_norm", "l1_norm_grad", "l2_norm_grad", "softmax_cross_entropy_loss_forward",
- * "softmax_cross_entropy_loss_backward" (int64 targets, VALID reduction).
- * `dims` holds the entry point's sizes in its own order: (N, C) for the two
- * LayerNorm ops, (N, G, D, S) for GroupNorm, (N, C, S) for BatchNorm, (N, S, C)
+ * "softmax_cross_entropy_loss_backward" (int64 targets, VALID reduction),
+ * "rms_norm" and "rms_norm_grad" (with a residual), "rms_norm_quant" (N, C, group),
+ * "topk_distillation_loss_forward", "topk_distillation_loss_backward" (N, C, K; int64
+ * classes, a VALID mean), "draft_verify" (B, K, C; int64 tokens, a sampled draft).
+ * `dims` holds the entry point's sizes in its own order: those named above, (N, C) for the
+ * LayerNorm and RMSNorm ops, (N, G, D, S) for GroupNorm, (N, C, S) for BatchNorm, (N, S, C)
  * for the rest; `layout` matters where the entry point takes one.
  * Returns the length of the text written to `buf` (truncated to buf_bytes - 1),
  * or a negative dragon_hip_status for an unknown op or a shape the entry point

@@ -1,0 +1,135 @@
+"""The operators of language models without a GPU: what the entry points refuse before anything is
+enqueued, the scratch they ask for, and the plain forms the GPU tests compare with."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from dragon_amd import _lib, kernels as K
+from tests import language_ops as L
+
+P = [ctypes.c_void_p((i + 1) << 32) for i in range(12)]  # distinct, never read
+EINVAL, EDTYPE, ESCRATCH = -1, -2, -3
+BIG = 1 << 40
+
+
+def test_rms_norm_refusals():
+    f = _lib.lib().dragon_hip_rms_norm
+    call = lambda dtype=1, N=4, C=8, x=P[0], r=P[1], g=P[2], h=P[3], rs=P[4], y=P[5]: f(
+        dtype, N, C, 1e-5, x, r, g, h, rs, y, None)
+    assert call(N=-1) == EINVAL and call(C=0) == EINVAL and call(C=1 << 31) == EINVAL and call(N=1 << 31) == EINVAL
+    assert call(x=None) == EINVAL and call(g=None) == EINVAL and call(y=None) == EINVAL
+    assert call(y=P[3]) == EINVAL  # y and h in one buffer
+    assert call(dtype=4) == EDTYPE and call(dtype=-1) == EDTYPE
+    assert call(N=0, x=None, y=None) == 0
+
+
+def test_rms_norm_quant_refusals():
+    f = _lib.lib().dragon_hip_rms_norm_quant
+    call = lambda dtype=1, N=4, C=8, group=0, x=P[0], q=P[5], s=P[6]: f(
+        dtype, N, C, group, 1e-5, x, P[1], P[2], P[3], P[4], q, s, None)
+    assert call(dtype=3) == EDTYPE and call(dtype=9) == EDTYPE
+    for group in (-1, 1, 16, 48, 512):
+        assert call(group=group) == EINVAL
+    assert call(x=None) == EINVAL and call(q=None) == EINVAL and call(s=None) == EINVAL
+    assert call(N=-1) == EINVAL and call(C=0) == EINVAL and call(C=1 << 31) == EINVAL
+    assert call(N=0) == 0
+
+
+def test_rms_norm_grad_refusals():
+    lib = _lib.lib()
+    call = lambda dtype=1, N=4, C=8, h=P[0], dg=P[5], dx=P[6], ws=P[7], nbytes=BIG: lib.dragon_hip_rms_norm_grad(
+        dtype, N, C, h, P[1], P[2], P[3], P[4], dg, dx, ws, nbytes, None)
+    need = lib.dragon_hip_rms_norm_grad_scratch_bytes(1, 4, 8)
+    assert need > 0
+    assert call(ws=None) == ESCRATCH and call(nbytes=need - 1) == ESCRATCH
+    assert call(h=None) == EINVAL and call(dg=None) == EINVAL and call(dx=None) == EINVAL and call(dx=P[0]) == EINVAL
+    assert call(N=-1) == EINVAL and call(C=0) == EINVAL and call(C=1 << 31) == EINVAL and call(N=1 << 31) == EINVAL
+    assert call(dtype=5) == EDTYPE
+    assert lib.dragon_hip_rms_norm_grad_scratch_bytes(1, 0, 8) == 0
+    assert lib.dragon_hip_rms_norm_grad_scratch_bytes(7, 4, 8) == 0
+
+
+def test_distillation_refusals():
+    lib = _lib.lib()
+    fwd = lambda dtype=1, it=5, N=4, C=8, k=2, t=1.0, norm=-1.0, x=P[0], st=P[3], loss=P[4], ws=P[5], nbytes=BIG: \
+        lib.dragon_hip_topk_distillation_loss_forward(dtype, it, N, C, k, t, norm, x, P[1], P[2], st, loss, ws, nbytes, None)
+    bwd = lambda dtype=1, it=5, N=4, C=8, k=2, t=1.0, norm=-1.0, x=P[0], st=P[3], dl=P[4], dx=P[5]: \
+        lib.dragon_hip_topk_distillation_loss_backward(dtype, it, N, C, k, t, norm, x, P[1], P[2], st, dl, dx, None)
+    for f in (fwd, bwd):
+        assert f(dtype=4) == EDTYPE and f(it=2) == EDTYPE
+        for bad in (dict(N=-1), dict(C=0), dict(k=0), dict(k=1025), dict(t=0.0), dict(t=-2.0), dict(t=float("nan")),
+                    dict(t=float("inf")), dict(norm=float("nan")), dict(x=None), dict(st=None), dict(C=1 << 31),
+                    dict(N=(1 << 31) - 1)):
+            assert f(**bad) == EINVAL, bad
+    assert fwd(loss=None) == EINVAL and bwd(dl=None) == EINVAL and bwd(dx=None) == EINVAL
+    assert fwd(ws=None) == ESCRATCH
+    assert fwd(nbytes=lib.dragon_hip_topk_distillation_loss_scratch_bytes(1, 4, 8) - 1) == ESCRATCH
+    assert bwd(N=0) == 0
+
+
+def test_draft_verify_refusals():
+    lib = _lib.lib()
+    call = lambda dtype=2, it=5, B=2, k=3, C=8, t=P[0], d=P[2], ua=P[4], us=P[5], tok=P[6], acc=P[7]: \
+        lib.dragon_hip_draft_verify(dtype, it, B, k, C, t, P[1], d, P[3], ua, us, tok, acc, P[8], BIG, None)
+    assert call(dtype=4) == EDTYPE and call(it=1) == EDTYPE
+    for bad in (dict(B=-1), dict(k=-1), dict(C=0), dict(C=1 << 31), dict(t=None), dict(d=None), dict(ua=None),
+                dict(us=None), dict(tok=None), dict(acc=None)):
+        assert call(**bad) == EINVAL, bad
+    assert call(B=0) == 0
+
+
+def test_every_operator_has_a_plan():
+    for op, dims in (("rms_norm", (8, 4096)), ("rms_norm_quant", (8, 4096, 128)), ("rms_norm_grad", (8, 4096)),
+                     ("topk_distillation_loss_forward", (8, 32000, 16)),
+                     ("topk_distillation_loss_backward", (8, 32000, 16)), ("draft_verify", (2, 4, 32000))):
+        assert "[" in K.plan_name(op, "bfloat16", dims)
+        with pytest.raises(ValueError):
+            K.plan_name(op, "bfloat16", (4, -1, 0))
+
+
+# ---------------------------------------------------------------- the plain forms themselves
+
+def test_plain_distillation_is_the_divergence_of_torch():
+    g = torch.Generator().manual_seed(0)
+    n, c, k, t = 5, 30, 4, 1.7
+    x = torch.randn(n, c, generator=g, dtype=torch.float64)
+    teacher = torch.randn(n, k, generator=g, dtype=torch.float64)
+    index = torch.stack([torch.randperm(c, generator=g)[:k] for _ in range(n)])
+    p = torch.softmax(teacher / t, 1)
+    want = (p * (p.log() - torch.log_softmax(x / t, 1).gather(1, index))).sum(1) * t * t
+    stats, rows, loss = L.distill_forward(t, "MEAN", x.numpy(), index.numpy(), teacher.numpy())
+    assert np.allclose(rows, want.numpy(), rtol=1e-13) and np.allclose(loss, want.mean().item(), rtol=1e-13)
+    x.requires_grad_()
+    p = torch.softmax(teacher / t, 1)
+    ((p * (p.log() - torch.log_softmax(x / t, 1).gather(1, index))).sum(1) * t * t).mean().backward()
+    dx, _, _ = L.distill_backward(t, "MEAN", x.detach().numpy(), index.numpy(), teacher.numpy(), stats, np.ones(1))
+    assert np.allclose(dx, x.grad.numpy(), rtol=1e-12, atol=1e-15)
+
+
+def test_plain_rms_norm_gradient_is_that_of_torch():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(4, 9, generator=g, dtype=torch.float64, requires_grad=True)
+    gamma = (torch.rand(9, generator=g, dtype=torch.float64) + 0.5).requires_grad_()
+    dy, dh = torch.randn(4, 9, generator=g, dtype=torch.float64), torch.randn(4, 9, generator=g, dtype=torch.float64)
+    y = x / torch.sqrt(x.square().mean(1, keepdim=True) + 1e-5) * gamma
+    ((y * dy).sum() + (x * dh).sum()).backward()
+    _, rs, want = L.rms_norm(x.detach().numpy(), None, gamma.detach().numpy(), 1e-5)
+    assert np.allclose(want, y.detach().numpy(), rtol=1e-13)
+    dx, dg = L.rms_norm_grad(x.detach().numpy(), rs, gamma.detach().numpy(), dy.numpy(), dh.numpy())
+    assert np.allclose(dx, x.grad.numpy(), rtol=1e-12, atol=1e-14) and np.allclose(dg, gamma.grad.numpy(), rtol=1e-12)
+
+
+def test_plain_verification_follows_the_target():
+    """Accepted and drawn first tokens together have the target's distribution: 40000 draws, five classes. A
+    class's share is off by more than 5 standard deviations (at most 0.0125) about once in a million."""
+    rng = np.random.default_rng(2)
+    p, q = np.array([0.4, 0.3, 0.2, 0.1, 0.0]), np.array([0.1, 0.2, 0.3, 0.2, 0.2])
+    B = 40000
+    drafted = rng.choice(5, (B, 1), p=q)
+    target = np.broadcast_to(np.stack([p, p]), (B, 2, 5))
+    tokens, n = L.draft_verify(target, np.broadcast_to(q, (B, 1, 5)), drafted, None, rng.random((B, 1)), rng.random(B))
+    share = np.bincount(tokens[:, 0], minlength=5) / B
+    assert np.abs(share - p).max() < 0.0125 and share[4] == 0
