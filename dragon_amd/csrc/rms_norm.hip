@@ -49,6 +49,27 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int n, const float (&v)[
   }
 }
 
+// The codes of a tile's packet, v times `inv`. The packet that was moved back writes only the
+// elements that are its own: those before may belong to a group of another scale.
+template <bool kRagged, int kVec>
+__device__ __forceinline__ void tile_codes(uint8_t* p, int dup, bool on, float inv, const float (&v)[kVec]) {
+  float w[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) w[e] = v[e] * inv;
+  if (!on) return;
+  if (kRagged && dup > 0) {
+    const uint32_t lo = e4m3x4(w[0], w[1], w[2], w[3]);
+    uint32_t hi = 0;
+    if constexpr (kVec == 8) hi = e4m3x4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      if (e >= dup) p[e] = static_cast<uint8_t>((e < 4 ? lo : hi) >> (8 * (e & 3)));
+    }
+  } else {
+    store_codes<kVec>(p, kVec, w);
+  }
+}
+
 // Largest value over `lanes` neighbouring lanes (a power of two, aligned).
 __device__ __forceinline__ float cluster_max(float v, int lanes) {
   for (int o = 1; o < lanes; o <<= 1) v = MaxOp()(v, __shfl_xor(v, o, kWaveSize));
@@ -148,10 +169,265 @@ __global__ __launch_bounds__(kLoopThreads) void rms_norm_rows_looped(
   }
 }
 
+// ------------------------------------------------------------------ rows held in registers
+
+// Workgroup sizes: rows of up to a wavefront's threads share one of 256 threads.
+constexpr int tile_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// The packets of a row that a thread of a group of kTPR holds: packet s * kTPR + lane in slot s.
+// Where rows are not whole aligned packets (kRagged), a row's last packet is moved back to end
+// with the row: every access is a whole packet inside the row, and the `dup` elements it shares
+// with the packet before it are left out of sums and written twice with the same values.
+template <typename T, int kTPR, int kVPT, bool kRagged>
+struct RowPackets {
+  static constexpr int kVec = IO<T>::kVec;
+  int col[kVPT], dup[kVPT];
+  bool on[kVPT];
+  __device__ __forceinline__ explicit RowPackets(int C) {
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) {
+      const int nominal = (s * kTPR + static_cast<int>(threadIdx.x) % kTPR) * kVec;
+      on[s] = nominal < C;
+      col[s] = on[s] ? nominal : 0;
+      dup[s] = 0;
+      if (kRagged && on[s] && nominal + kVec > C) {
+        col[s] = C - kVec;
+        dup[s] = nominal - col[s];
+      }
+    }
+  }
+  __device__ __forceinline__ bool counts(int s, int e) const { return !kRagged || e >= dup[s]; }
+  // Slots without a packet hold the row's first: they are masked where they are used.
+  __device__ __forceinline__ void load(const T* row, u32x4 (&p)[kVPT]) const {
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) {
+      if constexpr (kRagged) {
+        p[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_unaligned*>(row + col[s]));
+      } else {
+        p[s] = load_packet(row + col[s]);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int s, const typename IO<T>::Acc (&v)[kVec]) const {
+    if constexpr (kRagged) {
+      store_packet_unaligned(row + col[s], IO<T>::pack(v));
+    } else {
+      store_packet(row + col[s], IO<T>::pack(v));
+    }
+  }
+  __device__ __forceinline__ void params(const typename IO<T>::Acc* gamma, int s,
+                                         typename IO<T>::Acc (&g)[kVec]) const {
+    if constexpr (kRagged) {
+      load_params_ragged<kVec>(gamma + col[s], kVec, g);
+    } else {
+      load_params<kVec>(gamma + col[s], g);
+    }
+  }
+};
+
+// All-reduce over the kTPR threads of a row: lanes of one wavefront, or whole wavefronts through
+// LDS with one barrier. Rows alternate between two sets of `slots`, so that the barrier of one
+// row keeps the next but one from overwriting what is still being read.
+template <int kTPR, typename A, typename Op>
+__device__ __forceinline__ A row_allreduce(A v, Op op, A* slots) {
+  if constexpr (kTPR < kWaveSize) {
+#pragma unroll
+    for (int o = kTPR / 2; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, kWaveSize));
+    return v;
+  } else {
+    v = wave_allreduce(v, op);
+    if constexpr (kTPR == kWaveSize) return v;
+    constexpr int kWaves = kTPR / kWaveSize;
+    A* mine = slots + threadIdx.x / kTPR * kWaves;
+    if ((threadIdx.x & (kWaveSize - 1)) == 0) mine[threadIdx.x % kTPR / kWaveSize] = v;
+    __syncthreads();
+    A r = mine[0];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) r = op(r, mine[i]);
+    return r;
+  }
+}
+
+enum RmsOut { kPlain = 0, kRowScale = 1, kGroupScale = 2 };
+
+// One read of x and residual, one write of h and y. Workgroups stay and walk the rows, so that
+// gamma is loaded once into registers (of tiles of up to two packets per thread), and the next
+// row is requested before the current one is summed. Every element of a row is loaded before the
+// row's first store: outputs may lie on inputs.
+template <typename T, int kTPR, int kVPT, bool kRagged, bool kResidual, int kOut>
+__global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
+    const int64_t N, const int C, const typename IO<T>::Acc eps, const T* x, const T* residual,
+    const typename IO<T>::Acc* gamma, T* h, typename IO<T>::Acc* rsig, T* y, const int group,
+    const int groups, uint8_t* q, float* scale) {
+  using A = typename IO<T>::Acc;
+  constexpr int kVec = IO<T>::kVec;
+  constexpr int kThreads = tile_threads(kTPR), kRows = kThreads / kTPR;
+  constexpr bool kAhead = kVPT <= 2;  // wider tiles leave no registers for gamma and the next row
+  __shared__ A slots[2][2][kThreads / kWaveSize];
+  const RowPackets<T, kTPR, kVPT, kRagged> tile(C);
+  const A inv_c = A(1) / A(C);
+  A g[kVPT][kVec];
+  if constexpr (kAhead) {
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) tile.params(gamma, s, g[s]);
+  }
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR;
+  u32x4 px[kVPT], pr[kVPT];
+  tile.load(x + (row < N ? row : 0) * C, px);
+  if constexpr (kResidual) tile.load(residual + (row < N ? row : 0) * C, pr);
+  int turn = 0;
+  // the trip count is the same for every row of a workgroup: the reductions hold barriers
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < N; base += step) {
+    const bool valid = row < N;
+    A v[kVPT][kVec];
+    A sum = A(0);
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) {
+      IO<T>::unpack(px[s], v[s]);
+      if constexpr (kResidual) {
+        A r[kVec];
+        IO<T>::unpack(pr[s], r);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[s][e] += r[e];
+      }
+      A part = A(0);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) part += tile.counts(s, e) ? v[s][e] * v[s][e] : A(0);
+      sum += tile.on[s] ? part : A(0);
+    }
+    const int64_t next = row + step;
+    if constexpr (kAhead) {
+      tile.load(x + (next < N ? next : 0) * C, px);
+      if constexpr (kResidual) tile.load(residual + (next < N ? next : 0) * C, pr);
+    }
+    sum = row_allreduce<kTPR>(sum, SumOp(), slots[turn][0]);
+    const A rs = acc_rsqrt_exact(sum * inv_c + eps);
+    if (valid && threadIdx.x % kTPR == 0 && rsig) rsig[row] = rs;
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) {
+      if (h && valid && tile.on[s]) tile.store(h + row * C, s, v[s]);
+      if constexpr (!kAhead) tile.params(gamma, s, g[s]);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[s][e] = v[s][e] * rs * g[s][e];
+      if constexpr (kOut == kPlain) {
+        if (valid && tile.on[s]) tile.store(y + row * C, s, v[s]);
+      } else {
+        float part = 0.f;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) part = MaxOp()(part, tile.counts(s, e) ? fabsf(v[s][e]) : 0.f);
+        part = tile.on[s] ? part : 0.f;
+        if constexpr (kOut == kRowScale) {
+          top = MaxOp()(top, part);
+        } else {
+          // a group wider than the row stays inside the row's own lanes
+          const int lanes = group / kVec < kTPR ? group / kVec : kTPR;
+          const float amax = MaxOp()(cluster_max(part, lanes), kAmaxFloor);
+          const int nominal = tile.col[s] + tile.dup[s];
+          if (valid && tile.on[s] && nominal % group == 0) scale[row * groups + nominal / group] = amax / kFp8Max;
+          tile_codes<kRagged>(q + row * C + tile.col[s], tile.dup[s], valid && tile.on[s], kFp8Max / amax, v[s]);
+        }
+      }
+    }
+    if constexpr (kOut == kRowScale) {
+      const float amax = MaxOp()(row_allreduce<kTPR>(top, MaxOp(), slots[turn][1]), kAmaxFloor);
+      if (valid && threadIdx.x % kTPR == 0) scale[row] = amax / kFp8Max;
+#pragma unroll
+      for (int s = 0; s < kVPT; ++s)
+        tile_codes<kRagged>(q + row * C + tile.col[s], tile.dup[s], valid && tile.on[s], kFp8Max / amax, v[s]);
+    }
+    row = next;
+    turn ^= 1;
+    if constexpr (!kAhead) {
+      tile.load(x + (row < N ? row : 0) * C, px);
+      if constexpr (kResidual) tile.load(residual + (row < N ? row : 0) * C, pr);
+    }
+  }
+}
+
+// Calls LAUNCH(threads per row, packets per thread) for rows of `packets`: the fewest threads
+// that hold the row with up to two packets each, four on the largest workgroup.
+#define DRAGON_HIP_RMS_SWITCH_2(packets, LAUNCH)  \
+  if (packets <= 8) LAUNCH(8, 1)                  \
+  else if (packets <= 16) LAUNCH(16, 1)           \
+  else if (packets <= 32) LAUNCH(32, 1)           \
+  else if (packets <= 64) LAUNCH(64, 1)           \
+  else if (packets <= 128) LAUNCH(64, 2)          \
+  else if (packets <= 256) LAUNCH(128, 2)         \
+  else if (packets <= 512) LAUNCH(256, 2)         \
+  else if (packets <= 1024) LAUNCH(512, 2)        \
+  else LAUNCH(1024, 2)
+#define DRAGON_HIP_RMS_SWITCH(packets, LAUNCH) \
+  if (packets > 2048) LAUNCH(1024, 4)          \
+  else DRAGON_HIP_RMS_SWITCH_2(packets, LAUNCH)
+constexpr int64_t kMaxTilePackets = 4096;
+
+template <typename T, int kTPR, int kVPT, bool kRagged, bool kResidual, int kOut>
+int launch_rms_tile(int64_t N, int64_t C, float eps, const void* x, const void* residual,
+                    const void* gamma, void* h, void* rsig, void* y, int64_t group, int64_t groups,
+                    void* q, void* scale, hipStream_t stream) {
+  using A = typename IO<T>::Acc;
+  auto kernel = rms_norm_rows<T, kTPR, kVPT, kRagged, kResidual, kOut>;
+  constexpr int kThreads = tile_threads(kTPR);
+  const int64_t want = ceil_div(N, kThreads / kTPR);
+  const int64_t resident = resident_grid(kernel, kThreads, 0);
+  note_number("threads_per_row", kTPR);
+  note_number("packets", kVPT);
+  hipLaunchKernelGGL((rms_norm_rows<T, kTPR, kVPT, kRagged, kResidual, kOut>),
+                     dim3(static_cast<unsigned>(want < resident ? want : resident)), dim3(kThreads), 0,
+                     stream, N, static_cast<int>(C), A(eps), static_cast<const T*>(x),
+                     static_cast<const T*>(residual), static_cast<const A*>(gamma), static_cast<T*>(h),
+                     static_cast<A*>(rsig), static_cast<T*>(y), static_cast<int>(group),
+                     static_cast<int>(groups), static_cast<uint8_t*>(q), static_cast<float*>(scale));
+  return status_of_launch();
+}
+
+template <typename T, bool kRagged, bool kResidual, int kOut>
+int launch_rms_tiles(int64_t N, int64_t C, float eps, const void* x, const void* residual,
+                     const void* gamma, void* h, void* rsig, void* y, int64_t group, int64_t groups,
+                     void* q, void* scale, hipStream_t stream) {
+  const int64_t packets = ceil_div(C, IO<T>::kVec);
+#define LAUNCH(TPR, VPT)                                                                            \
+  return launch_rms_tile<T, TPR, VPT, kRagged, kResidual, kOut>(N, C, eps, x, residual, gamma, h, rsig, \
+                                                                y, group, groups, q, scale, stream);
+  DRAGON_HIP_RMS_SWITCH(packets, LAUNCH)
+#undef LAUNCH
+}
+
+// Whether rows of C elements fit the tiles: up to 4096 packets, and one at least where the last
+// packet is moved back.
+template <typename T>
+bool rms_tiles_fit(int64_t C) {
+  return C >= IO<T>::kVec && ceil_div(C, IO<T>::kVec) <= kMaxTilePackets;
+}
+
+template <typename T, int kOut>
+int launch_rms_rows(int64_t N, int64_t C, float eps, const void* x, const void* residual,
+                    const void* gamma, void* h, void* rsig, void* y, int64_t group, int64_t groups,
+                    void* q, void* scale, hipStream_t stream) {
+  // a null pointer counts as aligned; codes are written 8 or 4 bytes at a time
+  const bool regular = C % IO<T>::kVec == 0 && aligned16(x) && aligned16(residual) && aligned16(gamma) &&
+      aligned16(h) && aligned16(y) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+#define LAUNCH(RAGGED, RESIDUAL)                                                                     \
+  return launch_rms_tiles<T, RAGGED, RESIDUAL, kOut>(N, C, eps, x, residual, gamma, h, rsig, y, group, \
+                                                     groups, q, scale, stream);
+  if (regular) {
+    if (residual) LAUNCH(false, true) else LAUNCH(false, false)
+  } else {
+    if (residual) LAUNCH(true, true) else LAUNCH(true, false)
+  }
+#undef LAUNCH
+}
+
 template <typename T>
 int launch_rms_norm(int64_t N, int64_t C, float eps, const void* x, const void* residual,
                     const void* gamma, void* h, void* rsig, void* y, hipStream_t stream) {
   using A = typename IO<T>::Acc;
+  if (rms_tiles_fit<T>(C)) {
+    return launch_rms_rows<T, kPlain>(N, C, eps, x, residual, gamma, h, rsig, y, 0, 0, nullptr, nullptr,
+                                      stream);
+  }
   hipLaunchKernelGGL((rms_norm_rows_looped<T, false>), dim3(loop_grid(N)), dim3(kLoopThreads), 0,
                      stream, N, C, A(eps), static_cast<const T*>(x), static_cast<const T*>(residual),
                      static_cast<const A*>(gamma), static_cast<T*>(h), static_cast<A*>(rsig),
@@ -164,12 +440,19 @@ template <typename T>
 int launch_rms_norm_quant(int64_t N, int64_t C, int64_t group, float eps, const void* x,
                           const void* residual, const void* gamma, void* h, void* rsig, void* q,
                           void* scale, hipStream_t stream) {
+  const int64_t groups = group ? ceil_div(C, group) : static_cast<int64_t>(1);
+  if (rms_tiles_fit<T>(C)) {
+    if (group == 0)
+      return launch_rms_rows<T, kRowScale>(N, C, eps, x, residual, gamma, h, rsig, nullptr, group, groups,
+                                           q, scale, stream);
+    return launch_rms_rows<T, kGroupScale>(N, C, eps, x, residual, gamma, h, rsig, nullptr, group, groups,
+                                           q, scale, stream);
+  }
   hipLaunchKernelGGL((rms_norm_rows_looped<T, true>), dim3(loop_grid(N)), dim3(kLoopThreads), 0,
                      stream, N, C, eps, static_cast<const T*>(x), static_cast<const T*>(residual),
                      static_cast<const float*>(gamma), static_cast<T*>(h), static_cast<float*>(rsig),
                      static_cast<T*>(nullptr), static_cast<int>(group),
-                     group ? ceil_div(C, group) : static_cast<int64_t>(1), static_cast<uint8_t*>(q),
-                     static_cast<float*>(scale));
+                     groups, static_cast<uint8_t*>(q), static_cast<float*>(scale));
   return status_of_launch();
 }
 
@@ -251,16 +534,168 @@ __global__ __launch_bounds__(kColThreads) void rms_norm_grad_cols(
   }
 }
 
-// dgamma = the chunks' sums, added in order.
+// One read of h, dy and dh, one write of dx, and the column sums in the registers of workgroups
+// that stay and walk the rows: a thread owns the same columns of every row it meets. The groups
+// of a workgroup add theirs in LDS, in order, and each workgroup leaves one row of partial sums.
+constexpr int grad_threads(int tpr) { return tpr <= 512 ? 512 : 1024; }
+template <typename T, int kTPR, int kVPT, bool kRagged, bool kThrough>
+__global__ __launch_bounds__(grad_threads(kTPR), 4) void rms_norm_grad_rows(
+    const int64_t N, const int C, const T* h, const typename IO<T>::Acc* rsig,
+    const typename IO<T>::Acc* gamma, const T* dy, const T* dh, typename IO<T>::Acc* partial, T* dx) {
+  using A = typename IO<T>::Acc;
+  constexpr int kVec = IO<T>::kVec;
+  constexpr int kThreads = grad_threads(kTPR), kRows = kThreads / kTPR;
+  constexpr bool kAhead = kVPT <= 2;
+  __shared__ A slots[2][kThreads / kWaveSize];
+  // gamma of the thread's columns, then the sums of the workgroup's groups: 16-byte words, those of
+  // neighbouring lanes side by side
+  constexpr int kPer = 16 / sizeof(A), kWords = kVec / kPer;
+  __shared__ u32x4 shared[kVPT * kWords * kTPR];
+  const RowPackets<T, kTPR, kVPT, kRagged> tile(C);
+  const A inv_c = A(1) / A(C);
+  const int lane = static_cast<int>(threadIdx.x) % kTPR, mine = static_cast<int>(threadIdx.x) / kTPR;
+  auto word_at = [&](int s, int w) -> u32x4& { return shared[(s * kWords + w) * kTPR + lane]; };
+  auto read_words = [&](int s, A(&v)[kVec]) {
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      A part[kPer];
+      IO<A>::unpack(word_at(s, w), part);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[w * kPer + e] = part[e];
+    }
+  };
+  auto write_words = [&](int s, const A(&v)[kVec]) {
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      A part[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) part[e] = v[w * kPer + e];
+      word_at(s, w) = IO<A>::pack(part);
+    }
+  };
+  A acc[kVPT][kVec];
+#pragma unroll
+  for (int s = 0; s < kVPT; ++s) {
+    if (mine == 0) {
+      A g[kVec];
+      tile.params(gamma, s, g);
+      write_words(s, g);
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) acc[s][e] = A(0);
+  }
+  __syncthreads();
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR;
+  u32x4 ph[kVPT], py[kVPT], pd[kVPT];
+  A rs_next;
+  auto request = [&](int64_t r) {
+    r = r < N ? r : 0;
+    tile.load(h + r * C, ph);
+    tile.load(dy + r * C, py);
+    if constexpr (kThrough) tile.load(dh + r * C, pd);
+    rs_next = rsig[r];
+  };
+  request(row);
+  int turn = 0;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < N; base += step) {
+    const bool valid = row < N;
+    const A rs = rs_next;
+    u32x4 ch[kVPT], cy[kVPT], cd[kVPT];
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) {
+      ch[s] = ph[s], cy[s] = py[s];
+      if constexpr (kThrough) cd[s] = pd[s];
+    }
+    A dot = A(0);
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) {
+      A a[kVec], b[kVec], g[kVec];
+      IO<T>::unpack(ch[s], a);
+      IO<T>::unpack(cy[s], b);
+      read_words(s, g);
+      A part = A(0);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const A t = b[e] * a[e];
+        part += tile.counts(s, e) ? t * g[e] : A(0);
+        acc[s][e] += valid ? t * rs : A(0);  // what is shared with another packet is not written
+      }
+      dot += tile.on[s] ? part : A(0);
+    }
+    const int64_t next = row + step;
+    if constexpr (kAhead) request(next);
+    dot = row_allreduce<kTPR>(dot, SumOp(), slots[turn]);
+    const A c = dot * inv_c * rs * rs;
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) {
+      A a[kVec], b[kVec], d[kVec], g[kVec];
+      IO<T>::unpack(ch[s], a);
+      IO<T>::unpack(cy[s], b);
+      read_words(s, g);
+      if constexpr (kThrough) {
+        IO<T>::unpack(cd[s], d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) d[e] = A(0);
+      }
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) d[e] += rs * (b[e] * g[e] - a[e] * c);
+      if (valid && tile.on[s]) tile.store(dx + row * C, s, d);
+    }
+    row = next;
+    turn ^= 1;
+    if constexpr (!kAhead) request(row);
+  }
+  // one group after the other adds its sums; the last of them holds the workgroup's
+  for (int r = 0; kRows > 1 && r < kRows; ++r) {
+    __syncthreads();
+    if (mine != r) continue;
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) {
+      if (r > 0) {
+        A before[kVec];
+        read_words(s, before);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) acc[s][e] += before[e];
+      }
+      if (r + 1 < kRows) write_words(s, acc[s]);
+    }
+  }
+  if (mine != kRows - 1) return;
+  A* out = partial + static_cast<int64_t>(blockIdx.x) * C;
+#pragma unroll
+  for (int s = 0; s < kVPT; ++s) {
+    if (!tile.on[s]) continue;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      if (tile.counts(s, e)) out[tile.col[s] + e] = acc[s][e];
+    }
+  }
+}
+
+// dgamma = the sums of the partial rows: 16 words of a row by each of 64 groups of threads, which
+// take every 64th row and are then added in order.
+constexpr int kJoinThreads = 1024, kJoinWords = 16, kJoinGroups = kJoinThreads / kJoinWords;
 template <typename A>
-__global__ __launch_bounds__(kColThreads) void rms_norm_grad_join(const int64_t C, const int64_t chunks,
-                                                                  const A* __restrict__ partial,
-                                                                  A* __restrict__ dgamma) {
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kColThreads + threadIdx.x;
-  if (col >= C) return;
+__global__ __launch_bounds__(kJoinThreads) void rms_norm_grad_join(const int64_t C, const int64_t rows,
+                                                                   const A* __restrict__ partial,
+                                                                   A* __restrict__ dgamma) {
+  __shared__ A lds[kJoinGroups][kJoinWords + 1];
+  const int word = threadIdx.x % kJoinWords, group = threadIdx.x / kJoinWords;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kJoinWords + word;
   A sum = A(0);
-  for (int64_t p = 0; p < chunks; ++p) sum += partial[p * C + col];
-  dgamma[col] = sum;
+  if (col < C) {
+#pragma unroll 4
+    for (int64_t p = group; p < rows; p += kJoinGroups) sum += partial[p * C + col];
+  }
+  lds[group][word] = sum;
+  __syncthreads();
+  // a wavefront per word (16 of them): lane g holds the sum of group g
+  const int w = threadIdx.x / kWaveSize, lane = threadIdx.x % kWaveSize;
+  const A total = wave_allreduce(lds[lane][w], SumOp());
+  if (lane == 0 && static_cast<int64_t>(blockIdx.x) * kJoinWords + w < C)
+    dgamma[static_cast<int64_t>(blockIdx.x) * kJoinWords + w] = total;
 }
 
 struct GradCols {
@@ -276,11 +711,52 @@ inline GradCols plan_grad_cols(int64_t N, int64_t C, int vec) {
   return p;
 }
 
+// Rows that the register tiles hold: their workgroups (two of 512 threads or one of 1024 per
+// compute unit, by registers), each of which leaves a row of partial sums.
+// Four packets of 16-bit elements per thread (three tensors' and as many sums) do not fit the
+// registers of 1024 threads.
+template <typename T>
+bool grad_tiles_fit(int64_t C) {
+  return C >= IO<T>::kVec && ceil_div(C, IO<T>::kVec) <= (sizeof(T) == 2 ? kMaxTilePackets / 2 : kMaxTilePackets);
+}
+template <typename T>
+int64_t grad_grid(int64_t N, int64_t C) {
+  const int64_t packets = ceil_div(C, IO<T>::kVec);
+  int tpr = 0;
+#define TAKE(TPR, VPT) tpr = TPR;
+  DRAGON_HIP_RMS_SWITCH(packets, TAKE)
+#undef TAKE
+  const int threads = grad_threads(tpr);
+  const int64_t want = ceil_div(N, threads / tpr);
+  const int64_t most = static_cast<int64_t>(num_cus()) * (threads == 512 ? 2 : 1);
+  return want < most ? want : most;
+}
+
 template <typename T>
 size_t grad_scratch_bytes(int64_t N, int64_t C) {
   using A = typename IO<T>::Acc;
+  if (grad_tiles_fit<T>(C)) return static_cast<size_t>(grad_grid<T>(N, C)) * C * sizeof(A);
   const GradCols p = plan_grad_cols(N, C, IO<T>::kVec);
   return static_cast<size_t>(N + p.chunks * C) * sizeof(A);
+}
+
+template <typename T, bool kRagged, bool kThrough>
+void launch_grad_tiles(int64_t N, int64_t C, unsigned grid, const T* h, const typename IO<T>::Acc* rsig,
+                       const typename IO<T>::Acc* gamma, const T* dy, const T* dh,
+                       typename IO<T>::Acc* partial, T* dx, hipStream_t stream) {
+  const int64_t packets = ceil_div(C, IO<T>::kVec);
+#define LAUNCH(TPR, VPT)                                                                            \
+  {                                                                                                 \
+    hipLaunchKernelGGL((rms_norm_grad_rows<T, TPR, VPT, kRagged, kThrough>), dim3(grid),            \
+                       dim3(grad_threads(TPR)), 0, stream, N, static_cast<int>(C), h, rsig, gamma, dy, \
+                       dh, partial, dx);                                                            \
+  }
+  if constexpr (sizeof(T) == 2) {
+    DRAGON_HIP_RMS_SWITCH_2(packets, LAUNCH)
+  } else {
+    DRAGON_HIP_RMS_SWITCH(packets, LAUNCH)
+  }
+#undef LAUNCH
 }
 
 template <typename T>
@@ -289,22 +765,37 @@ int launch_rms_norm_grad(int64_t N, int64_t C, const void* h, const void* rsig, 
                          size_t scratch_bytes, hipStream_t stream) {
   using A = typename IO<T>::Acc;
   if (N > 0 && (!scratch || scratch_bytes < grad_scratch_bytes<T>(N, C))) return DRAGON_HIP_ESCRATCH;
-  const GradCols p = plan_grad_cols(N, C, IO<T>::kVec);
-  A* coef = static_cast<A*>(scratch);
-  A* partial = coef + N;
-  if (N > 0) {
+  const T* hp = static_cast<const T*>(h);
+  const T* yp = static_cast<const T*>(dy);
+  const T* dp = static_cast<const T*>(dh);
+  const A* rp = static_cast<const A*>(rsig);
+  const A* gp = static_cast<const A*>(gamma);
+  T* xp = static_cast<T*>(dx);
+  A* partial = static_cast<A*>(scratch);
+  int64_t rows = 0;  // of partial sums
+  if (N > 0 && grad_tiles_fit<T>(C)) {
+    rows = grad_grid<T>(N, C);
+    const unsigned grid = static_cast<unsigned>(rows);
+    const bool regular = C % IO<T>::kVec == 0 && aligned16(h) && aligned16(gamma) && aligned16(dy) &&
+        aligned16(dh) && aligned16(dx);
+    if (regular && dh) launch_grad_tiles<T, false, true>(N, C, grid, hp, rp, gp, yp, dp, partial, xp, stream);
+    else if (regular) launch_grad_tiles<T, false, false>(N, C, grid, hp, rp, gp, yp, dp, partial, xp, stream);
+    else if (dh) launch_grad_tiles<T, true, true>(N, C, grid, hp, rp, gp, yp, dp, partial, xp, stream);
+    else launch_grad_tiles<T, true, false>(N, C, grid, hp, rp, gp, yp, dp, partial, xp, stream);
+  } else if (N > 0) {
+    const GradCols p = plan_grad_cols(N, C, IO<T>::kVec);
+    A* coef = partial;
+    partial += N;
+    rows = p.chunks;
     hipLaunchKernelGGL((rms_norm_grad_dots<T>), dim3(loop_grid(N)), dim3(kLoopThreads), 0, stream, N, C,
-                       static_cast<const T*>(h), static_cast<const A*>(rsig),
-                       static_cast<const A*>(gamma), static_cast<const T*>(dy), coef);
+                       hp, rp, gp, yp, coef);
     const dim3 grid(static_cast<unsigned>(ceil_div(C, static_cast<int64_t>(IO<T>::kVec) * kColThreads)),
                     static_cast<unsigned>(p.chunks));
     hipLaunchKernelGGL((rms_norm_grad_cols<T>), grid, dim3(kColThreads), 0, stream, N, C,
-                       p.rows_per_chunk, static_cast<const T*>(h), static_cast<const A*>(rsig),
-                       static_cast<const A*>(gamma), static_cast<const T*>(dy),
-                       static_cast<const T*>(dh), coef, partial, static_cast<T*>(dx));
+                       p.rows_per_chunk, hp, rp, gp, yp, dp, coef, partial, xp);
   }
-  hipLaunchKernelGGL((rms_norm_grad_join<A>), dim3(static_cast<unsigned>(ceil_div(C, kColThreads))),
-                     dim3(kColThreads), 0, stream, C, p.chunks, partial, static_cast<A*>(dgamma));
+  hipLaunchKernelGGL((rms_norm_grad_join<A>), dim3(static_cast<unsigned>(ceil_div(C, kJoinWords))),
+                     dim3(kJoinThreads), 0, stream, C, rows, partial, static_cast<A*>(dgamma));
   return status_of_launch();
 }
 
