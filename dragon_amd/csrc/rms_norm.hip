@@ -683,19 +683,22 @@ __global__ __launch_bounds__(kJoinThreads) void rms_norm_grad_join(const int64_t
                                                                    A* __restrict__ dgamma) {
   __shared__ A lds[kJoinGroups][kJoinWords + 1];
   const int word = threadIdx.x % kJoinWords, group = threadIdx.x / kJoinWords;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kJoinWords + word;
-  A sum = A(0);
-  if (col < C) {
-#pragma unroll 4
-    for (int64_t p = group; p < rows; p += kJoinGroups) sum += partial[p * C + col];
-  }
-  lds[group][word] = sum;
-  __syncthreads();
-  // a wavefront per word (16 of them): lane g holds the sum of group g
   const int w = threadIdx.x / kWaveSize, lane = threadIdx.x % kWaveSize;
-  const A total = wave_allreduce(lds[lane][w], SumOp());
-  if (lane == 0 && static_cast<int64_t>(blockIdx.x) * kJoinWords + w < C)
-    dgamma[static_cast<int64_t>(blockIdx.x) * kJoinWords + w] = total;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kJoinWords; base < C;
+       base += static_cast<int64_t>(gridDim.x) * kJoinWords) {
+    const int64_t col = base + word;
+    A sum = A(0);
+    if (col < C) {
+#pragma unroll 4
+      for (int64_t p = group; p < rows; p += kJoinGroups) sum += partial[p * C + col];
+    }
+    lds[group][word] = sum;
+    __syncthreads();
+    // a wavefront per word (16 of them): lane g holds the sum of group g
+    const A total = wave_allreduce(lds[lane][w], SumOp());
+    if (lane == 0 && base + w < C) dgamma[base + w] = total;
+    __syncthreads();
+  }
 }
 
 struct GradCols {
@@ -794,7 +797,7 @@ int launch_rms_norm_grad(int64_t N, int64_t C, const void* h, const void* rsig, 
     hipLaunchKernelGGL((rms_norm_grad_cols<T>), grid, dim3(kColThreads), 0, stream, N, C,
                        p.rows_per_chunk, hp, rp, gp, yp, dp, coef, partial, xp);
   }
-  hipLaunchKernelGGL((rms_norm_grad_join<A>), dim3(static_cast<unsigned>(ceil_div(C, kJoinWords))),
+  hipLaunchKernelGGL((rms_norm_grad_join<A>), dim3(row_grid(C, kJoinWords)),
                      dim3(kJoinThreads), 0, stream, C, rows, partial, static_cast<A*>(dgamma));
   return status_of_launch();
 }
