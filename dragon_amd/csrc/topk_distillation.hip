@@ -16,7 +16,11 @@
 namespace dragon_hip {
 namespace {
 
-constexpr int kMaxK = 1024;
+constexpr int kMaxK = 1024;  // entries that a workgroup holds
+#ifndef SEGMAX
+#define SEGMAX 2048
+#endif
+
 
 // How exponentials of logits at a temperature are taken. `scale` turns a logit into the domain
 // that running maxima m are held in; term(x) is exp of the logit x relative to m, shrink(d) the
@@ -112,12 +116,6 @@ __device__ __forceinline__ bool group_any(bool v) {
   else return __syncthreads_or(v);
 }
 
-// Whether an entry is listed: its class is in the row and its teacher logit is not -inf.
-template <typename A, typename IndexT>
-__device__ __forceinline__ bool entry_listed(IndexT index, A logit, int64_t C) {
-  return index >= 0 && static_cast<int64_t>(index) < C && logit != acc_neg_inf<A>();
-}
-
 // A row cut at the 16-byte boundaries of its memory: `head` elements, `packets` whole aligned
 // packets, `tail` elements. Head and tail are shorter than a packet.
 template <typename T>
@@ -133,76 +131,117 @@ struct RowCut {
   }
 };
 
-// The teacher's side and the loss of a row, from the pair of its logits, by the kTPR threads of
-// its group.
+// The teacher's entries of a row in the registers of its group, four to a thread at most (more would
+// cost a kernel's occupancy for rare K): entry k belongs to thread k % kTPR, in slot k / kTPR.
+// Everything is requested at once.
+constexpr int kWaveK = 4 * kWaveSize;  // entries that a wavefront holds
 template <typename T, typename IndexT, int kTPR>
-__device__ __forceinline__ void finish_row(const int64_t row, const int64_t C, const int K,
+struct Entries {
+  using A = typename IO<T>::Acc;
+  static constexpr int kSlots = 4;
+  int cls[kSlots];  // -1: not listed
+  A z[kSlots];      // teacher's logit / t
+  __device__ __forceinline__ void load(int64_t row, int64_t C, int K, A inv_t, const IndexT* index,
+                                       const A* teacher) {
+    const int lane = static_cast<int>(threadIdx.x) % kTPR;
+    IndexT c[kSlots];
+    A l[kSlots];
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      c[i] = IndexT(-1);
+      l[i] = acc_neg_inf<A>();
+      if (i * kTPR + lane < K) {
+        c[i] = index[row * K + i * kTPR + lane];
+        l[i] = teacher[row * K + i * kTPR + lane];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      const bool listed = c[i] >= 0 && static_cast<int64_t>(c[i]) < C && l[i] != acc_neg_inf<A>();
+      cls[i] = listed ? static_cast<int>(c[i]) : -1;
+      z[i] = listed ? l[i] * inv_t : acc_neg_inf<A>();
+    }
+  }
+  __device__ __forceinline__ bool any() const {
+    bool on = false;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) on |= cls[i] >= 0;
+    return group_any<kTPR>(on);
+  }
+  // Their maximum (which passes over NaN) and the sum of their exponentials (which keeps it).
+  __device__ __forceinline__ ExpSum<A> sum(A (*slots)[kTPR / kWaveSize]) const {
+    A m = acc_neg_inf<A>();
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) m = MaxOp()(m, z[i]);
+    m = group_reduce<kTPR>(m, MaxOp(), slots[0]);
+    A total = A(0);
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) total += cls[i] >= 0 ? acc_exp(z[i] - m) : A(0);
+    return {m, group_reduce<kTPR>(total, SumOp(), slots[1])};
+  }
+};
+
+// The loss of a row from the pair of its logits, by the kTPR threads of its group.
+template <typename T, typename IndexT, int kTPR>
+__device__ __forceinline__ void finish_row(const int64_t row, const int64_t C,
                                            const typename IO<T>::Acc inv_t,
-                                           const typename IO<T>::Acc t2, const T* x, const IndexT* index,
-                                           const typename IO<T>::Acc* teacher,
+                                           const typename IO<T>::Acc t2, const T* x,
+                                           const Entries<T, IndexT, kTPR>& entries,
                                            const ExpSum<typename IO<T>::Acc> run,
                                            typename IO<T>::Acc* stats, typename IO<T>::Acc* loss,
                                            typename IO<T>::Acc (*slots)[kTPR / kWaveSize]) {
   using A = typename IO<T>::Acc;
-  const int lane = static_cast<int>(threadIdx.x) % kTPR;
-  A m = acc_neg_inf<A>();  // the maximum passes over NaN; the sum keeps it
-  for (int k = lane; k < K; k += kTPR) {
-    const A logit = teacher[row * K + k];
-    if (entry_listed(index[row * K + k], logit, C)) m = MaxOp()(m, logit * inv_t);
-  }
-  m = group_reduce<kTPR>(m, MaxOp(), slots[0]);
-  A total = A(0);
-  for (int k = lane; k < K; k += kTPR) {
-    const A logit = teacher[row * K + k];
-    if (entry_listed(index[row * K + k], logit, C)) total += acc_exp(logit * inv_t - m);
-  }
-  total = group_reduce<kTPR>(total, SumOp(), slots[1]);
-  const A log_total = acc_log(total);
+  constexpr int kSlots = Entries<T, IndexT, kTPR>::kSlots;
+  A xk[kSlots];
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i)
+    xk[i] = entries.cls[i] >= 0 ? IO<T>::load1(x + row * C + entries.cls[i]) * inv_t : A(0);
+  const ExpSum<A> t = entries.sum(slots);
+  const A log_total = acc_log(t.s);
   // a row of nothing but -inf has no distribution
   const A lse = run.m == acc_neg_inf<A>() ? A(__builtin_nanf("")) : ExpMath<T>::log_of(run.m, run.s);
   A part = A(0);
-  for (int k = lane; k < K; k += kTPR) {
-    const A logit = teacher[row * K + k];
-    const IndexT cls = index[row * K + k];
-    if (entry_listed(cls, logit, C)) {
-      const A log_p = logit * inv_t - m - log_total;
-      const A p = acc_exp(log_p);
-      const A xk = IO<T>::load1(x + row * C + static_cast<int64_t>(cls)) * inv_t;
-      if (p != A(0)) part += p * (log_p - xk + lse);
-    }
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    if (entries.cls[i] < 0) continue;
+    const A log_p = entries.z[i] - t.m - log_total;
+    const A p = acc_exp(log_p);
+    if (p != A(0)) part += p * (log_p - xk[i] + lse);
   }
   part = group_reduce<kTPR>(part, SumOp(), slots[2]);
-  if (lane == 0) {
+  if (threadIdx.x % kTPR == 0) {
     stats[row] = lse;
     loss[row] = part * t2;
   }
 }
 
-// A group of kTPR threads (a wavefront, four of them to a workgroup, or a workgroup) reads segment
-// blockIdx.y of a row. Where a row is one segment, it finishes the row; otherwise it leaves its
-// pair. Rows that list nothing are not read.
+// A group of kTPR threads (a wavefront, four of them to a workgroup, or a workgroup) reads a segment
+// of a row, the segments of a row by neighbouring groups. Where a row is one segment, it finishes
+// the row; otherwise it leaves its pair. Rows that list nothing are not read.
 constexpr int kSegmentThreads = 256;
 template <typename T, typename IndexT, int kTPR, bool kWhole>
 __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
-    const int64_t N, const int64_t C, const int K, const int64_t segment_packets,
+    const int64_t N, const int64_t C, const int K, const uint32_t segments, const int64_t segment_packets,
     const typename IO<T>::Acc inv_t, const typename IO<T>::Acc t2, const T* __restrict__ x,
     const IndexT* __restrict__ index, const typename IO<T>::Acc* __restrict__ teacher,
     typename IO<T>::Acc* __restrict__ stats, typename IO<T>::Acc* __restrict__ loss,
-    ExpSum<typename IO<T>::Acc>* __restrict__ pairs) {
+    ExpSum<typename IO<T>::Acc>* __restrict__ pairs, const bool reduced) {
   using A = typename IO<T>::Acc;
   constexpr int kVec = IO<T>::kVec;
+  if (!reduced && blockIdx.x == 0 && threadIdx.x == 0) stats[N] = A(1);  // the divisor of single losses
   constexpr int kUnroll = 4;
   __shared__ A slots[5][kTPR / kWaveSize];
   constexpr int kRows = kSegmentThreads / kTPR;
   const int lane = static_cast<int>(threadIdx.x) % kTPR;
   const A scale = ExpMath<T>::scale(inv_t);
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; row < N;
-       row += static_cast<int64_t>(gridDim.x) * kRows) {
-    bool listed = false;
-    for (int k = lane; k < K; k += kTPR)
-      listed |= entry_listed(index[row * K + k], teacher[row * K + k], C);
-    if (!group_any<kTPR>(listed)) {
-      if (lane == 0 && blockIdx.y == 0) {
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; item < N * segments;
+       item += static_cast<int64_t>(gridDim.x) * kRows) {
+    const int64_t row = kWhole ? item : item / segments;
+    const uint32_t segment = kWhole ? 0 : static_cast<uint32_t>(item - row * segments);
+    Entries<T, IndexT, kTPR> entries;
+    entries.load(row, C, K, inv_t, index, teacher);
+    if (!entries.any()) {
+      if (lane == 0 && segment == 0) {
         stats[row] = -acc_neg_inf<A>();
         loss[row] = A(0);
       }
@@ -212,9 +251,9 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
     const RowCut<T> cut(xr, C);
     const T* body = xr + cut.head;
     ExpSum<A> run = {acc_neg_inf<A>(), A(0)};
-    int64_t p = static_cast<int64_t>(blockIdx.y) * segment_packets;
+    int64_t p = segment * segment_packets;
     const int64_t end = p + segment_packets < cut.packets ? p + segment_packets : cut.packets;
-    if (blockIdx.y == 0) {
+    if (segment == 0) {
       if (lane < cut.head) take_one<T>(IO<T>::load1(xr + lane), scale, run);
       if (lane < cut.tail) take_one<T>(IO<T>::load1(body + cut.packets * kVec + lane), scale, run);
     }
@@ -234,57 +273,57 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
     }
     run = group_join<T, kTPR>(run, slots);
     if constexpr (kWhole) {
-      finish_row<T, IndexT, kTPR>(row, C, K, inv_t, t2, x, index, teacher, run, stats, loss, slots + 2);
+      finish_row<T, IndexT, kTPR>(row, C, inv_t, t2, x, entries, run, stats, loss, slots + 2);
     } else if (lane == 0) {
-      pairs[row * gridDim.y + blockIdx.y] = run;
+      pairs[item] = run;
     }
     if constexpr (kTPR > kWaveSize) __syncthreads();  // slots are reused by the next row
   }
 }
 
-// Joins the pairs of a row's segments and finishes the row: a wavefront per row.
-template <typename T, typename IndexT>
+// Joins the pairs of a row's segments and finishes the row: a wavefront per row, or a workgroup.
+template <typename T, typename IndexT, int kTPR>
 __global__ __launch_bounds__(kSegmentThreads) void distill_forward_join(
     const int64_t N, const int64_t C, const int K, const int segments, const typename IO<T>::Acc inv_t,
     const typename IO<T>::Acc t2, const T* __restrict__ x, const IndexT* __restrict__ index,
     const typename IO<T>::Acc* __restrict__ teacher, typename IO<T>::Acc* __restrict__ stats,
     typename IO<T>::Acc* __restrict__ loss, const ExpSum<typename IO<T>::Acc>* __restrict__ pairs) {
   using A = typename IO<T>::Acc;
-  constexpr int kRows = kSegmentThreads / kWaveSize;
-  const int lane = static_cast<int>(threadIdx.x) % kWaveSize;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kWaveSize; row < N;
+  constexpr int kRows = kSegmentThreads / kTPR;
+  __shared__ A slots[5][kTPR / kWaveSize];
+  const int lane = static_cast<int>(threadIdx.x) % kTPR;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; row < N;
        row += static_cast<int64_t>(gridDim.x) * kRows) {
-    bool listed = false;
-    for (int k = lane; k < K; k += kWaveSize)
-      listed |= entry_listed(index[row * K + k], teacher[row * K + k], C);
-    if (!__any(listed)) continue;  // written by the row's first segment
+    Entries<T, IndexT, kTPR> entries;
+    entries.load(row, C, K, inv_t, index, teacher);
+    if (!entries.any()) continue;  // written by the row's first segment, which left no pair
     ExpSum<A> run = {acc_neg_inf<A>(), A(0)};
-    for (int i = lane; i < segments; i += kWaveSize) {
+    for (int i = lane; i < segments; i += kTPR) {
       const ExpSum<A> other = pairs[row * segments + i];
       const A m = MaxOp()(run.m, other.m);
       const A base = finite_base(m);
       run = {m, run.s * ExpMath<T>::shrink(run.m - base) + other.s * ExpMath<T>::shrink(other.m - base)};
     }
-    run = group_join<T, kWaveSize>(run, static_cast<A(*)[1]>(nullptr));
-    finish_row<T, IndexT, kWaveSize>(row, C, K, inv_t, t2, x, index, teacher, run, stats, loss,
-                                     static_cast<A(*)[1]>(nullptr));
+    run = group_join<T, kTPR>(run, slots);
+    finish_row<T, IndexT, kTPR>(row, C, inv_t, t2, x, entries, run, stats, loss, slots + 2);
+    if constexpr (kTPR > kWaveSize) __syncthreads();  // slots are reused by the next row
   }
 }
 
-// How a row is cut into segments. A wavefront takes rows of up to 512 packets whole. Longer rows are
+// How a row is cut into segments. A wavefront takes rows of up to 512 packets whole, if it holds
+// the entries. Longer rows are
 // read by workgroups, 4096 packets (16 per thread) at most at a time, and 1024 at least where
 // there are too few rows to give every compute unit eight workgroups.
 struct SegmentPlan {
   bool wave_rows;
   int64_t segments, packets;  // per row, per segment
 };
-inline SegmentPlan plan_segments(int64_t N, int64_t C, int vec) {
+inline SegmentPlan plan_segments(int64_t N, int64_t C, int64_t K, int vec) {
   const int64_t packets = ceil_div(C, vec);
-  if (packets <= 512) return {true, 1, packets};
-  const int64_t fewest = ceil_div(packets, 4096), most = ceil_div(packets, 1024);
+  if (packets <= 512) return {K <= kWaveK, 1, packets};
+  const int64_t fewest = ceil_div(packets, SEGMAX), most = ceil_div(packets, 1024);
   int64_t segments = ceil_div(static_cast<int64_t>(num_cus()) * 8, N > 0 ? N : 1);
   segments = segments < fewest ? fewest : (segments > most ? most : segments);
-  if (segments > 32768) segments = 32768;  // a launch's second extent holds 65535
   const int64_t each = ceil_div(packets, segments);
   return {false, ceil_div(packets, each), each};
 }
@@ -297,9 +336,14 @@ __global__ __launch_bounds__(kLoopThreads) void distill_reduce(const int64_t N, 
                                                                A* __restrict__ stats, A* __restrict__ loss) {
   __shared__ A slots[2][kLoopWaves];
   A sum = A(0), count = A(0);
-  for (int64_t i = threadIdx.x; i < N; i += kLoopThreads) {
-    sum += rows[i];
-    count += stats[i] != -acc_neg_inf<A>() ? A(1) : A(0);
+  constexpr int kAtOnce = 8;  // loads in flight: the loop is all latency
+  for (int64_t base = 0; base < N; base += kAtOnce * kLoopThreads) {
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int64_t i = base + k * kLoopThreads + threadIdx.x;
+      sum += i < N ? rows[i] : A(0);
+      count += i < N && stats[i] != -acc_neg_inf<A>() ? A(1) : A(0);
+    }
   }
   sum = block_allreduce<kLoopWaves>(sum, SumOp(), slots[0]);
   count = block_allreduce<kLoopWaves>(count, SumOp(), slots[1]);
@@ -320,7 +364,7 @@ int launch_forward(int64_t N, int64_t C, int64_t K, float temperature, float nor
                    hipStream_t stream) {
   using A = typename IO<T>::Acc;
   const bool reduce = normalizer != 0.f;
-  const SegmentPlan plan = plan_segments(N, C, IO<T>::kVec);
+  const SegmentPlan plan = plan_segments(N, C, K, IO<T>::kVec);
   ExpSum<A>* pairs = static_cast<ExpSum<A>*>(scratch);
   A* rows = reduce ? static_cast<A*>(scratch) + 2 * N * plan.segments : static_cast<A*>(loss);
   const T* xp = static_cast<const T*>(x);
@@ -331,24 +375,31 @@ int launch_forward(int64_t N, int64_t C, int64_t K, float temperature, float nor
   const int k = static_cast<int>(K);
   if (N > 0) {
     const dim3 block(kSegmentThreads), waves(row_grid(N, kSegmentThreads / kWaveSize));
-    const dim3 grid(row_grid(N, 1), static_cast<unsigned>(plan.segments));
+    const dim3 grid(row_grid(N * plan.segments, 1));
+    const uint32_t segments = static_cast<uint32_t>(plan.segments);
     if (plan.wave_rows) {
       hipLaunchKernelGGL((distill_forward_segments<T, IndexT, kWaveSize, true>), waves, block, 0, stream, N,
-                         C, k, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs);
+                         C, k, segments, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs, reduce);
     } else if (plan.segments == 1) {
       hipLaunchKernelGGL((distill_forward_segments<T, IndexT, kSegmentThreads, true>), grid, block, 0,
-                         stream, N, C, k, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs);
+                         stream, N, C, k, segments, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs, reduce);
     } else {
       hipLaunchKernelGGL((distill_forward_segments<T, IndexT, kSegmentThreads, false>), grid, block, 0,
-                         stream, N, C, k, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs);
-      hipLaunchKernelGGL((distill_forward_join<T, IndexT>), waves, block, 0, stream, N, C, k,
-                         static_cast<int>(plan.segments), inv_t, t2, xp, ip, tp, sp, rows, pairs);
+                         stream, N, C, k, segments, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs, reduce);
+      if (K <= kWaveK) {
+        hipLaunchKernelGGL((distill_forward_join<T, IndexT, kWaveSize>), waves, block, 0, stream, N, C, k,
+                           static_cast<int>(plan.segments), inv_t, t2, xp, ip, tp, sp, rows, pairs);
+      } else {
+        hipLaunchKernelGGL((distill_forward_join<T, IndexT, kSegmentThreads>), dim3(row_grid(N, 1)), block, 0,
+                           stream, N, C, k, static_cast<int>(plan.segments), inv_t, t2, xp, ip, tp, sp, rows,
+                           pairs);
+      }
     }
   }
   if (reduce) {
     hipLaunchKernelGGL((distill_reduce<A>), dim3(1), dim3(kLoopThreads), 0, stream, N, normalizer, rows,
                        sp, static_cast<A*>(loss));
-  } else {
+  } else if (N == 0) {
     hipLaunchKernelGGL((distill_no_reduction<A>), dim3(1), dim3(1), 0, stream, N, sp);
   }
   return status_of_launch();
@@ -356,124 +407,131 @@ int launch_forward(int64_t N, int64_t C, int64_t K, float temperature, float nor
 
 // ------------------------------------------------------------------ gradient
 
-// A workgroup writes the gradient of a segment of a row: the softmax everywhere, then, behind a
-// barrier, the listed classes of the segment again with the teacher's share taken off. The logits
-// of those are read before the first store, so that dx may lie on x.
-template <typename T, typename IndexT>
+// Orders what the threads of a row's group wrote: a workgroup's barrier, or, where the group is one
+// wavefront, whose memory operations stay in order, a fence for the compiler.
+template <int kTPR>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (kTPR == kWaveSize) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+
+// A group of kTPR threads holds a segment of a row, kVPT packets each, and writes its gradient:
+// the softmax everywhere, then the listed classes of the segment again with the teacher's share
+// taken off. The segment is requested before the teacher's side is computed, which hides behind
+// it, and every logit is read before the first store, so that dx may lie on x. Small segments
+// keep what all workgroups read and write at a time close together in memory: [4096, 131072]
+// bf16 in segments of 4096, 2048 and 1024 packets walked by 256 threads took 374, 354 and 330 us.
+template <typename T, typename IndexT, int kTPR, int kVPT>
 __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
-    const int64_t N, const int64_t C, const int K, const int64_t segment_packets,
+    const int64_t N, const int64_t C, const int K, const uint32_t segments, const int64_t segment_packets,
     const typename IO<T>::Acc inv_t, const typename IO<T>::Acc temperature, const bool per_row, const T* x,
     const IndexT* index, const typename IO<T>::Acc* teacher, const typename IO<T>::Acc* stats,
     const typename IO<T>::Acc* dl, T* dx) {
   using A = typename IO<T>::Acc;
   using Math = ExpMath<T>;
-  constexpr int kVec = IO<T>::kVec, kThreads = kSegmentThreads, kWaves = kThreads / kWaveSize;
-  constexpr int kUnroll = 4, kMine = kMaxK / kThreads;  // entries of a thread
-  __shared__ A slots[2][kWaves];
-  __shared__ int classes[kMaxK];
-  __shared__ A shares[kMaxK];
-  const int lane = threadIdx.x;
-  for (int64_t row = blockIdx.x; row < N; row += gridDim.x) {
+  constexpr int kVec = IO<T>::kVec, kRows = kSegmentThreads / kTPR;
+  constexpr int kSlots = Entries<T, IndexT, kTPR>::kSlots;
+  __shared__ A slots[2][kTPR / kWaveSize];
+  extern __shared__ u32x4 entry_lds[];  // per group: the shares of K entries, then their classes
+  const int lane = static_cast<int>(threadIdx.x) % kTPR, group = static_cast<int>(threadIdx.x) / kTPR;
+  const int padded = (K + 3) / 4 * 4;
+  A* shares = reinterpret_cast<A*>(entry_lds) + static_cast<int64_t>(group) * padded;
+  int* classes = reinterpret_cast<int*>(reinterpret_cast<A*>(entry_lds) + kRows * padded) + group * padded;
+  const A scale = Math::scale(inv_t);
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kRows + group; item < N * segments;
+       item += static_cast<int64_t>(gridDim.x) * kRows) {
+    const int64_t row = item / segments;
+    const uint32_t segment = static_cast<uint32_t>(item - row * segments);
     const A lse = stats[row];
     T* out = dx + row * C;
     const T* in = x + row * C;
     const RowCut<T> cut(out, C);  // stores are aligned; loads are where x and dx lie alike
-    const bool first = blockIdx.y == 0;
-    int64_t p = static_cast<int64_t>(blockIdx.y) * segment_packets;
-    const int64_t end = p + segment_packets < cut.packets ? p + segment_packets : cut.packets;
+    const bool first = segment == 0;
+    const int64_t tail_at = cut.head + cut.packets * kVec + lane;
+    const int64_t begin = segment * segment_packets;
+    const int64_t end = begin + segment_packets < cut.packets ? begin + segment_packets : cut.packets;
     if (lse == -acc_neg_inf<A>()) {  // ignored
       A zero[kVec];
 #pragma unroll
       for (int e = 0; e < kVec; ++e) zero[e] = A(0);
       if (first && lane < cut.head) IO<T>::store1(out + lane, A(0));
-      if (first && lane < cut.tail) IO<T>::store1(out + cut.head + cut.packets * kVec + lane, A(0));
-      for (p += lane; p < end; p += kThreads) pack_store<T>(out + cut.head + p * kVec, zero);
+      if (first && lane < cut.tail) IO<T>::store1(out + tail_at, A(0));
+      for (int64_t p = begin + lane; p < end; p += kTPR) pack_store<T>(out + cut.head + p * kVec, zero);
       continue;
     }
+    u32x4 raw[kVPT];
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) {
+      const int64_t p = begin + s * kTPR + lane;
+      if (p < end) {
+        raw[s] = __builtin_nontemporal_load(
+            reinterpret_cast<const u32x4_unaligned*>(in + cut.head + p * kVec));
+      }
+    }
+    A head = A(0), tail = A(0);
+    if (first && lane < cut.head) head = IO<T>::load1(in + lane);
+    if (first && lane < cut.tail) tail = IO<T>::load1(in + tail_at);
+    // the teacher's shares
+    Entries<T, IndexT, kTPR> entries;
+    entries.load(row, C, K, inv_t, index, teacher);
     const A divisor = stats[N];
     const A w = dl[per_row ? row : 0] * temperature / (divisor > A(0.5) ? divisor : A(0.5));
-    const A scale = Math::scale(inv_t), base = Math::from_log(lse);
-    // the teacher's shares; entry k belongs to thread k % kThreads
-    A z[kMine], m = acc_neg_inf<A>();
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int k = i * kThreads + lane;
-      z[i] = acc_neg_inf<A>();
-      if (k < K) {
-        const IndexT cls = index[row * K + k];
-        const A logit = teacher[row * K + k];
-        const bool listed = entry_listed(cls, logit, C);
-        classes[k] = listed ? static_cast<int>(cls) : -1;
-        if (listed) {
-          z[i] = logit * inv_t;
-          m = MaxOp()(m, z[i]);
-        }
-      }
-    }
-    m = block_allreduce<kWaves>(m, MaxOp(), slots[0]);
-    A total = A(0);
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      z[i] = z[i] == acc_neg_inf<A>() ? A(0) : acc_exp(z[i] - m);
-      total += z[i];
-    }
-    total = block_allreduce<kWaves>(total, SumOp(), slots[1]);
+    const A base = Math::from_log(lse);
     // the listed classes of this segment; the row's head and tail are the first segment's
-    A kept[kMine];
-    bool here[kMine];
+    A kept[kSlots];
+    bool here[kSlots];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int k = i * kThreads + lane;
-      here[i] = false;
-      kept[i] = A(0);
-      if (k < K) {
-        shares[k] = z[i] / total;
-        const int64_t cls = classes[k];
-        const bool edge = cls < cut.head || cls >= cut.head + cut.packets * kVec;
-        here[i] = cls >= 0 && (edge ? first : cls >= cut.head + p * kVec && cls < cut.head + end * kVec);
-        if (here[i]) kept[i] = IO<T>::load1(in + cls);
+    for (int i = 0; i < kSlots; ++i) {
+      const int64_t cls = entries.cls[i];
+      const bool edge = cls < cut.head || cls >= cut.head + cut.packets * kVec;
+      here[i] = cls >= 0 && (edge ? first : cls >= cut.head + begin * kVec && cls < cut.head + end * kVec);
+      kept[i] = here[i] ? IO<T>::load1(in + cls) : A(0);
+    }
+    const ExpSum<A> t = entries.sum(slots);
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      const int k = i * kTPR + lane;
+      if (k < padded) {
+        classes[k] = entries.cls[i];
+        shares[k] = entries.cls[i] >= 0 ? acc_exp(entries.z[i] - t.m) / t.s : A(0);
       }
+      // its logit has arrived before another thread may write over it
+      asm volatile("" : "+v"(kept[i]));
     }
-    __syncthreads();
-    if (first) {
-      if (lane < cut.head) IO<T>::store1(out + lane, w * Math::term(IO<T>::load1(in + lane), scale, base));
-      const int64_t at = cut.head + cut.packets * kVec + lane;
-      if (lane < cut.tail) IO<T>::store1(out + at, w * Math::term(IO<T>::load1(in + at), scale, base));
+    group_sync<kTPR>();
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      if (!here[i]) continue;
+      A share = A(0);  // of every entry of this class
+      for (int k = 0; k < padded; k += 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) share += classes[k + j] == entries.cls[i] ? shares[k + j] : A(0);
+      }
+      kept[i] = w * (Math::term(kept[i], scale, base) - share);
     }
-    const T* src = in + cut.head;
-    T* dst = out + cut.head;
-    for (; p + kUnroll * kThreads <= end; p += kUnroll * kThreads) {
-      u32x4 raw[kUnroll];
+    if (first && lane < cut.head) IO<T>::store1(out + lane, w * Math::term(head, scale, base));
+    if (first && lane < cut.tail) IO<T>::store1(out + tail_at, w * Math::term(tail, scale, base));
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k)
-        raw[k] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4_unaligned*>(src + (p + k * kThreads + lane) * kVec));
-#pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
+    for (int s = 0; s < kVPT; ++s) {
+      const int64_t p = begin + s * kTPR + lane;
+      if (p < end) {
         A v[kVec];
-        IO<T>::unpack(raw[k], v);
+        IO<T>::unpack(raw[s], v);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) v[e] = w * Math::term(v[e], scale, base);
-        pack_store<T>(dst + (p + k * kThreads + lane) * kVec, v);
+        pack_store<T>(out + cut.head + p * kVec, v);
       }
     }
-    for (p += lane; p < end; p += kThreads) {
-      A v[kVec];
-      IO<T>::unpack(load_packet_unaligned(src + p * kVec), v);
+    group_sync<kTPR>();  // the second store of a listed class comes behind the first
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[e] = w * Math::term(v[e], scale, base);
-      pack_store<T>(dst + p * kVec, v);
+    for (int i = 0; i < kSlots; ++i) {
+      if (here[i]) IO<T>::store1(out + entries.cls[i], kept[i]);
     }
-    __syncthreads();  // the second store of a listed class comes behind the first
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      if (!here[i]) continue;
-      const int cls = classes[i * kThreads + lane];
-      A share = A(0);
-      for (int k = 0; k < K; ++k) share += classes[k] == cls ? shares[k] : A(0);
-      IO<T>::store1(out + cls, w * (Math::term(kept[i], scale, base) - share));
-    }
-    __syncthreads();  // classes and shares are reused by the next row
+    group_sync<kTPR>();  // the entries' LDS is reused by the next item
   }
 }
 
@@ -482,13 +540,26 @@ int launch_backward(int64_t N, int64_t C, int64_t K, float temperature, float no
                     const void* index, const void* teacher, const void* stats, const void* dl, void* dx,
                     hipStream_t stream) {
   using A = typename IO<T>::Acc;
-  const SegmentPlan plan = plan_segments(N, C, IO<T>::kVec);
-  hipLaunchKernelGGL((distill_backward_segments<T, IndexT>),
-                     dim3(row_grid(N, 1), static_cast<unsigned>(plan.segments)),
-                     dim3(kSegmentThreads), 0, stream, N, C, static_cast<int>(K), plan.packets,
-                     A(1) / A(temperature), A(temperature), normalizer == 0.f, static_cast<const T*>(x),
-                     static_cast<const IndexT*>(index), static_cast<const A*>(teacher),
-                     static_cast<const A*>(stats), static_cast<const A*>(dl), static_cast<T*>(dx));
+  const int64_t packets = ceil_div(C, IO<T>::kVec);
+  const size_t lds = static_cast<size_t>((K + 3) / 4 * 4) * (sizeof(A) + sizeof(int));
+#define LAUNCH(TPR, VPT, SEGMENTS, PACKETS)                                                          \
+  {                                                                                                  \
+    const int64_t segments = SEGMENTS;                                                               \
+    constexpr int kRows = kSegmentThreads / TPR;                                                     \
+    hipLaunchKernelGGL((distill_backward_segments<T, IndexT, TPR, VPT>),                             \
+                       dim3(row_grid(N * segments, kRows)), dim3(kSegmentThreads), lds * kRows, stream, \
+                       N, C, static_cast<int>(K), static_cast<uint32_t>(segments),                   \
+                       static_cast<int64_t>(PACKETS), A(1) / A(temperature), A(temperature),         \
+                       normalizer == 0.f, static_cast<const T*>(x), static_cast<const IndexT*>(index), \
+                       static_cast<const A*>(teacher), static_cast<const A*>(stats),                 \
+                       static_cast<const A*>(dl), static_cast<T*>(dx));                              \
+  }
+  // rows of up to 512 packets by a wavefront, if it holds the entries; longer ones in equal segments
+  // of 1024 at most
+  if (packets <= 256 && K <= kWaveK) LAUNCH(64, 4, 1, packets)
+  else if (packets <= 512 && K <= kWaveK) LAUNCH(64, 8, 1, packets)
+  else LAUNCH(256, 4, ceil_div(packets, 1024), ceil_div(packets, segments))
+#undef LAUNCH
   return status_of_launch();
 }
 
@@ -529,7 +600,7 @@ size_t dragon_hip_topk_distillation_loss_scratch_bytes(int dtype, int64_t N, int
   const size_t acc = dtype == DRAGON_HIP_F64 ? 8 : 4;
   const int vec = dtype == DRAGON_HIP_F64 ? 2 : (dtype == DRAGON_HIP_F32 ? 4 : 8);
   // a pair per segment, then a loss per row
-  return static_cast<size_t>(N) * (2 * plan_segments(N, C, vec).segments + 1) * acc;
+  return static_cast<size_t>(N) * (2 * plan_segments(N, C, kMaxK, vec).segments + 1) * acc;
 }
 
 int dragon_hip_topk_distillation_loss_forward(int dtype, int index_dtype, int64_t N, int64_t C,
