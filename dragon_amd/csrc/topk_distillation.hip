@@ -17,9 +17,6 @@ namespace dragon_hip {
 namespace {
 
 constexpr int kMaxK = 1024;  // entries that a workgroup holds
-#ifndef SEGMAX
-#define SEGMAX 2048
-#endif
 
 
 // How exponentials of logits at a temperature are taken. `scale` turns a logit into the domain
@@ -131,14 +128,14 @@ struct RowCut {
   }
 };
 
-// The teacher's entries of a row in the registers of its group, four to a thread at most (more would
-// cost a kernel's occupancy for rare K): entry k belongs to thread k % kTPR, in slot k / kTPR.
-// Everything is requested at once.
+// The teacher's entries of a row in the registers of its group, one or four to a thread (four
+// where K asks for them: they cost a kernel's occupancy): entry k belongs to thread k % kTPR, in
+// slot k / kTPR. Everything is requested at once.
 constexpr int kWaveK = 4 * kWaveSize;  // entries that a wavefront holds
-template <typename T, typename IndexT, int kTPR>
+template <typename T, typename IndexT, int kTPR, int kSlotsT>
 struct Entries {
   using A = typename IO<T>::Acc;
-  static constexpr int kSlots = 4;
+  static constexpr int kSlots = kSlotsT;
   int cls[kSlots];  // -1: not listed
   A z[kSlots];      // teacher's logit / t
   __device__ __forceinline__ void load(int64_t row, int64_t C, int K, A inv_t, const IndexT* index,
@@ -182,16 +179,15 @@ struct Entries {
 };
 
 // The loss of a row from the pair of its logits, by the kTPR threads of its group.
-template <typename T, typename IndexT, int kTPR>
+template <typename T, typename IndexT, int kTPR, int kSlots>
 __device__ __forceinline__ void finish_row(const int64_t row, const int64_t C,
                                            const typename IO<T>::Acc inv_t,
                                            const typename IO<T>::Acc t2, const T* x,
-                                           const Entries<T, IndexT, kTPR>& entries,
+                                           const Entries<T, IndexT, kTPR, kSlots>& entries,
                                            const ExpSum<typename IO<T>::Acc> run,
                                            typename IO<T>::Acc* stats, typename IO<T>::Acc* loss,
                                            typename IO<T>::Acc (*slots)[kTPR / kWaveSize]) {
   using A = typename IO<T>::Acc;
-  constexpr int kSlots = Entries<T, IndexT, kTPR>::kSlots;
   A xk[kSlots];
 #pragma unroll
   for (int i = 0; i < kSlots; ++i)
@@ -219,7 +215,7 @@ __device__ __forceinline__ void finish_row(const int64_t row, const int64_t C,
 // of a row, the segments of a row by neighbouring groups. Where a row is one segment, it finishes
 // the row; otherwise it leaves its pair. Rows that list nothing are not read.
 constexpr int kSegmentThreads = 256;
-template <typename T, typename IndexT, int kTPR, bool kWhole>
+template <typename T, typename IndexT, int kTPR, int kSlots, bool kWhole>
 __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
     const int64_t N, const int64_t C, const int K, const uint32_t segments, const int64_t segment_packets,
     const typename IO<T>::Acc inv_t, const typename IO<T>::Acc t2, const T* __restrict__ x,
@@ -238,7 +234,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
        item += static_cast<int64_t>(gridDim.x) * kRows) {
     const int64_t row = kWhole ? item : item / segments;
     const uint32_t segment = kWhole ? 0 : static_cast<uint32_t>(item - row * segments);
-    Entries<T, IndexT, kTPR> entries;
+    Entries<T, IndexT, kTPR, kSlots> entries;
     entries.load(row, C, K, inv_t, index, teacher);
     if (!entries.any()) {
       if (lane == 0 && segment == 0) {
@@ -273,7 +269,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
     }
     run = group_join<T, kTPR>(run, slots);
     if constexpr (kWhole) {
-      finish_row<T, IndexT, kTPR>(row, C, inv_t, t2, x, entries, run, stats, loss, slots + 2);
+      finish_row<T, IndexT, kTPR, kSlots>(row, C, inv_t, t2, x, entries, run, stats, loss, slots + 2);
     } else if (lane == 0) {
       pairs[item] = run;
     }
@@ -282,7 +278,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
 }
 
 // Joins the pairs of a row's segments and finishes the row: a wavefront per row, or a workgroup.
-template <typename T, typename IndexT, int kTPR>
+template <typename T, typename IndexT, int kTPR, int kSlots>
 __global__ __launch_bounds__(kSegmentThreads) void distill_forward_join(
     const int64_t N, const int64_t C, const int K, const int segments, const typename IO<T>::Acc inv_t,
     const typename IO<T>::Acc t2, const T* __restrict__ x, const IndexT* __restrict__ index,
@@ -294,7 +290,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_join(
   const int lane = static_cast<int>(threadIdx.x) % kTPR;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; row < N;
        row += static_cast<int64_t>(gridDim.x) * kRows) {
-    Entries<T, IndexT, kTPR> entries;
+    Entries<T, IndexT, kTPR, kSlots> entries;
     entries.load(row, C, K, inv_t, index, teacher);
     if (!entries.any()) continue;  // written by the row's first segment, which left no pair
     ExpSum<A> run = {acc_neg_inf<A>(), A(0)};
@@ -305,15 +301,16 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_join(
       run = {m, run.s * ExpMath<T>::shrink(run.m - base) + other.s * ExpMath<T>::shrink(other.m - base)};
     }
     run = group_join<T, kTPR>(run, slots);
-    finish_row<T, IndexT, kTPR>(row, C, inv_t, t2, x, entries, run, stats, loss, slots + 2);
+    finish_row<T, IndexT, kTPR, kSlots>(row, C, inv_t, t2, x, entries, run, stats, loss, slots + 2);
     if constexpr (kTPR > kWaveSize) __syncthreads();  // slots are reused by the next row
   }
 }
 
 // How a row is cut into segments. A wavefront takes rows of up to 512 packets whole, if it holds
 // the entries. Longer rows are
-// read by workgroups, 4096 packets (16 per thread) at most at a time, and 1024 at least where
-// there are too few rows to give every compute unit eight workgroups.
+// read by workgroups, 2048 packets (8 per thread) at most at a time (of [4096, 131072] bf16: 153 us;
+// 4096 packets 155, 1024 163, for the entries that each reads), and 1024 at least where there
+// are too few rows to give every compute unit eight workgroups.
 struct SegmentPlan {
   bool wave_rows;
   int64_t segments, packets;  // per row, per segment
@@ -321,7 +318,7 @@ struct SegmentPlan {
 inline SegmentPlan plan_segments(int64_t N, int64_t C, int64_t K, int vec) {
   const int64_t packets = ceil_div(C, vec);
   if (packets <= 512) return {K <= kWaveK, 1, packets};
-  const int64_t fewest = ceil_div(packets, SEGMAX), most = ceil_div(packets, 1024);
+  const int64_t fewest = ceil_div(packets, 2048), most = ceil_div(packets, 1024);
   int64_t segments = ceil_div(static_cast<int64_t>(num_cus()) * 8, N > 0 ? N : 1);
   segments = segments < fewest ? fewest : (segments > most ? most : segments);
   const int64_t each = ceil_div(packets, segments);
@@ -377,24 +374,33 @@ int launch_forward(int64_t N, int64_t C, int64_t K, float temperature, float nor
     const dim3 block(kSegmentThreads), waves(row_grid(N, kSegmentThreads / kWaveSize));
     const dim3 grid(row_grid(N * plan.segments, 1));
     const uint32_t segments = static_cast<uint32_t>(plan.segments);
+#define SEGMENTS(TPR, WHOLE, GRID)                                                                  \
+  if (K <= TPR) {                                                                                   \
+    hipLaunchKernelGGL((distill_forward_segments<T, IndexT, TPR, 1, WHOLE>), GRID, block, 0, stream, N, \
+                       C, k, segments, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs, reduce); \
+  } else {                                                                                          \
+    hipLaunchKernelGGL((distill_forward_segments<T, IndexT, TPR, 4, WHOLE>), GRID, block, 0, stream, N, \
+                       C, k, segments, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs, reduce); \
+  }
+#define JOIN(TPR, SLOTS, GRID)                                                                      \
+  hipLaunchKernelGGL((distill_forward_join<T, IndexT, TPR, SLOTS>), GRID, block, 0, stream, N, C, k, \
+                     static_cast<int>(plan.segments), inv_t, t2, xp, ip, tp, sp, rows, pairs);
     if (plan.wave_rows) {
-      hipLaunchKernelGGL((distill_forward_segments<T, IndexT, kWaveSize, true>), waves, block, 0, stream, N,
-                         C, k, segments, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs, reduce);
+      SEGMENTS(64, true, waves)
     } else if (plan.segments == 1) {
-      hipLaunchKernelGGL((distill_forward_segments<T, IndexT, kSegmentThreads, true>), grid, block, 0,
-                         stream, N, C, k, segments, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs, reduce);
+      SEGMENTS(256, true, grid)
     } else {
-      hipLaunchKernelGGL((distill_forward_segments<T, IndexT, kSegmentThreads, false>), grid, block, 0,
-                         stream, N, C, k, segments, plan.packets, inv_t, t2, xp, ip, tp, sp, rows, pairs, reduce);
-      if (K <= kWaveK) {
-        hipLaunchKernelGGL((distill_forward_join<T, IndexT, kWaveSize>), waves, block, 0, stream, N, C, k,
-                           static_cast<int>(plan.segments), inv_t, t2, xp, ip, tp, sp, rows, pairs);
+      SEGMENTS(256, false, grid)
+      if (K <= 64) {
+        JOIN(64, 1, waves)
+      } else if (K <= kWaveK) {
+        JOIN(64, 4, waves)
       } else {
-        hipLaunchKernelGGL((distill_forward_join<T, IndexT, kSegmentThreads>), dim3(row_grid(N, 1)), block, 0,
-                           stream, N, C, k, static_cast<int>(plan.segments), inv_t, t2, xp, ip, tp, sp, rows,
-                           pairs);
+        JOIN(256, 4, dim3(row_grid(N, 1)))
       }
     }
+#undef SEGMENTS
+#undef JOIN
   }
   if (reduce) {
     hipLaunchKernelGGL((distill_reduce<A>), dim3(1), dim3(kLoopThreads), 0, stream, N, normalizer, rows,
@@ -422,10 +428,14 @@ __device__ __forceinline__ void group_sync() {
 // A group of kTPR threads holds a segment of a row, kVPT packets each, and writes its gradient:
 // the softmax everywhere, then the listed classes of the segment again with the teacher's share
 // taken off. The segment is requested before the teacher's side is computed, which hides behind
-// it, and every logit is read before the first store, so that dx may lie on x. Small segments
-// keep what all workgroups read and write at a time close together in memory: [4096, 131072]
-// bf16 in segments of 4096, 2048 and 1024 packets walked by 256 threads took 374, 354 and 330 us.
-template <typename T, typename IndexT, int kTPR, int kVPT>
+// it, and every logit is read before the first store, so that dx may lie on x. Small segments, of
+// neighbouring workgroups, keep what is read and written at a time close together in memory:
+// [4096, 131072] bf16 took 374 and 354 us in segments of 4096 and 2048 packets, 346 in segments of
+// 1024 and 339 of 512 (a plain copy of its size by workgroups of this shape: 330), and 543 of 256,
+// where the teacher's side outweighs the segment. Taking the shares off in the registers of the
+// packets' owners instead of storing those classes again took 341 to 393 us, for more work
+// between the loads and the stores.
+template <typename T, typename IndexT, int kTPR, int kVPT, int kSlots>
 __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
     const int64_t N, const int64_t C, const int K, const uint32_t segments, const int64_t segment_packets,
     const typename IO<T>::Acc inv_t, const typename IO<T>::Acc temperature, const bool per_row, const T* x,
@@ -434,7 +444,6 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
   using A = typename IO<T>::Acc;
   using Math = ExpMath<T>;
   constexpr int kVec = IO<T>::kVec, kRows = kSegmentThreads / kTPR;
-  constexpr int kSlots = Entries<T, IndexT, kTPR>::kSlots;
   __shared__ A slots[2][kTPR / kWaveSize];
   extern __shared__ u32x4 entry_lds[];  // per group: the shares of K entries, then their classes
   const int lane = static_cast<int>(threadIdx.x) % kTPR, group = static_cast<int>(threadIdx.x) / kTPR;
@@ -476,7 +485,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
     if (first && lane < cut.head) head = IO<T>::load1(in + lane);
     if (first && lane < cut.tail) tail = IO<T>::load1(in + tail_at);
     // the teacher's shares
-    Entries<T, IndexT, kTPR> entries;
+    Entries<T, IndexT, kTPR, kSlots> entries;
     entries.load(row, C, K, inv_t, index, teacher);
     const A divisor = stats[N];
     const A w = dl[per_row ? row : 0] * temperature / (divisor > A(0.5) ? divisor : A(0.5));
@@ -542,11 +551,11 @@ int launch_backward(int64_t N, int64_t C, int64_t K, float temperature, float no
   using A = typename IO<T>::Acc;
   const int64_t packets = ceil_div(C, IO<T>::kVec);
   const size_t lds = static_cast<size_t>((K + 3) / 4 * 4) * (sizeof(A) + sizeof(int));
-#define LAUNCH(TPR, VPT, SEGMENTS, PACKETS)                                                          \
+#define LAUNCH(TPR, VPT, SLOTS, SEGMENTS, PACKETS)                                                   \
   {                                                                                                  \
     const int64_t segments = SEGMENTS;                                                               \
     constexpr int kRows = kSegmentThreads / TPR;                                                     \
-    hipLaunchKernelGGL((distill_backward_segments<T, IndexT, TPR, VPT>),                             \
+    hipLaunchKernelGGL((distill_backward_segments<T, IndexT, TPR, VPT, SLOTS>),                             \
                        dim3(row_grid(N * segments, kRows)), dim3(kSegmentThreads), lds * kRows, stream, \
                        N, C, static_cast<int>(K), static_cast<uint32_t>(segments),                   \
                        static_cast<int64_t>(PACKETS), A(1) / A(temperature), A(temperature),         \
@@ -555,10 +564,14 @@ int launch_backward(int64_t N, int64_t C, int64_t K, float temperature, float no
                        static_cast<const A*>(dl), static_cast<T*>(dx));                              \
   }
   // rows of up to 512 packets by a wavefront, if it holds the entries; longer ones in equal segments
-  // of 1024 at most
-  if (packets <= 256 && K <= kWaveK) LAUNCH(64, 4, 1, packets)
-  else if (packets <= 512 && K <= kWaveK) LAUNCH(64, 8, 1, packets)
-  else LAUNCH(256, 4, ceil_div(packets, 1024), ceil_div(packets, segments))
+  // of 512 packets at most, or of 1024 where each of them reads more than 64 entries
+  if (packets <= 256 && K <= 64) LAUNCH(64, 4, 1, 1, packets)
+  else if (packets <= 512 && K <= 64) LAUNCH(64, 8, 1, 1, packets)
+  else if (packets <= 256 && K <= kWaveK) LAUNCH(64, 4, 4, 1, packets)
+  else if (packets <= 512 && K <= kWaveK) LAUNCH(64, 8, 4, 1, packets)
+  else if (K <= 64) LAUNCH(256, 2, 1, ceil_div(packets, 512), ceil_div(packets, segments))
+  else if (K <= 256) LAUNCH(256, 4, 1, ceil_div(packets, 1024), ceil_div(packets, segments))
+  else LAUNCH(256, 4, 4, ceil_div(packets, 1024), ceil_div(packets, segments))
 #undef LAUNCH
   return status_of_launch();
 }
