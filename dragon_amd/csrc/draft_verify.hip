@@ -10,44 +10,63 @@
 // 64 bits, where another order moves them by parts in 10^16.
 #include <climits>
 
-#include "row_loop.h"
 #include "row_tile.h"
 #include "span.h"
 
 namespace dragon_hip {
 namespace {
 
-// A probability: anything negative or not finite counts as 0 (the maximum drops NaN).
-template <typename A>
-__device__ __forceinline__ double weight_of(A p) {
-  const A v = MaxOp()(p, A(0));
-  return static_cast<double>(v < -acc_neg_inf<A>() ? v : A(0));
+// A probability: anything negative or not finite counts as 0. One test for the class of positive
+// normal and subnormal numbers.
+__device__ __forceinline__ double weight_of(float p) {
+  return static_cast<double>(__builtin_amdgcn_classf(p, 0x180) ? p : 0.f);
+}
+__device__ __forceinline__ double weight_of(double p) { return __builtin_amdgcn_class(p, 0x180) ? p : 0.0; }
+
+template <typename IndexT>
+__device__ __forceinline__ int64_t length_of(const IndexT* lengths, int64_t b, int64_t K) {
+  if (!lengths) return K;
+  const int64_t len = static_cast<int64_t>(lengths[b]);
+  return len < 0 ? 0 : (len > K ? K : len);
 }
 
-// How many of a sequence's drafted tokens pass, found by one wavefront, 64 positions at a time:
-// the first lane that refuses ends it.
+// How many of a sequence's drafted tokens pass, and how many there are. Found by one wavefront, 64
+// positions at a time: the first lane that refuses ends it. What a position is judged by is
+// requested beside the length, not behind it.
+struct Verdict {
+  int64_t n, len;
+};
 template <typename T, typename IndexT>
-__device__ __forceinline__ int64_t count_accepted(const int64_t b, const int64_t K, const int64_t C,
-                                                  const int64_t len, const T* target, const T* draft,
-                                                  const IndexT* drafted, const float* u_accept) {
+__device__ __forceinline__ Verdict judge(const int64_t b, const int64_t K, const int64_t C, const T* target,
+                                         const T* draft, const IndexT* drafted, const IndexT* lengths,
+                                         const float* u_accept) {
   const int lane = threadIdx.x & (kWaveSize - 1);
-  for (int64_t first = 0; first < len; first += kWaveSize) {
+  int64_t len = K;
+  for (int64_t first = 0; first < K; first += kWaveSize) {
     const int64_t i = first + lane;
-    bool refuse = false;
-    if (i < len) {
-      const int64_t d = static_cast<int64_t>(drafted[b * K + i]);
-      refuse = true;
-      if (d >= 0 && d < C) {
-        const double p = weight_of(IO<T>::load1(target + (b * (K + 1) + i) * C + d));
-        const double q =
-            draft ? weight_of(IO<T>::load1(draft + (b * K + i) * C + d)) : 1.0;
-        refuse = !(static_cast<double>(u_accept[b * K + i]) * q < p);
-      }
+    int64_t d = -1;
+    float u = 0.f;
+    if (i < K) {
+      d = static_cast<int64_t>(drafted[b * K + i]);
+      u = u_accept[b * K + i];
     }
-    const unsigned long long refused = __ballot(refuse);
-    if (refused) return first + __builtin_ctzll(refused);
+    if (first == 0) len = length_of(lengths, b, K);
+    bool refuse = true;
+    if (d >= 0 && d < C) {
+      const double p = weight_of(IO<T>::load1(target + (b * (K + 1) + i) * C + d));
+      const double q = draft ? weight_of(IO<T>::load1(draft + (b * K + i) * C + d)) : 1.0;
+      refuse = !(static_cast<double>(u) * q < p);
+    }
+    const unsigned long long refused = __ballot(refuse || i >= len);
+    if (refused) return {first + __builtin_ctzll(refused), len};
   }
-  return len;
+  return {K, len};
+}
+
+// A packet that is read once: streams gain a tenth from the non-temporal hint.
+template <typename T>
+__device__ __forceinline__ u32x4 load_packet_once(const T* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_unaligned*>(p));
 }
 
 // The row that a sequence's token is drawn from: max(p - q, 0), with q a row of the draft, or all
@@ -59,318 +78,361 @@ struct SampleRow {
   const T* p;
   const T* q;
   int64_t spike;
-  // The kVec classes from `col`: their weights, and what the target alone gives them.
-  __device__ __forceinline__ void weigh(int64_t col, const A (&a)[kVec], const A (&b)[kVec],
-                                        double (&w)[kVec], double (&plain)[kVec]) const {
+  // The packet of classes from `at`. One that would reach behind the row's end is moved back to end
+  // with it: its first `dup` classes belong to the packet before and weigh nothing here.
+  struct Piece {
+    int64_t col;
+    int dup;
+    bool on;
+  };
+  static __device__ __forceinline__ Piece piece(int64_t at, int64_t end) {
+    const bool on = at < end;
+    const int64_t col = at + kVec > end && end >= kVec ? end - kVec : at;
+    return {on ? col : 0, on ? static_cast<int>(at - col) : kVec, on};
+  }
+  static __device__ __forceinline__ u32x4 packet(const T* row, const Piece& at, int64_t end) {
+    if (end < kVec) {  // rows shorter than a packet
+      A v[kVec];
+      load_span<T>(row, static_cast<int>(end), A(0), v);
+      return IO<T>::pack(v);
+    }
+    return load_packet_unaligned(row + at.col);
+  }
+  // The weights of a piece, given its packets. 9 operations per class, three of them in 64 bits, which
+  // the 8 bytes per class of 32-bit rows leave time for.
+  __device__ __forceinline__ void weigh(int64_t col, const u32x4 tp, const u32x4 tq, double (&w)[kVec]) const {
+    A a[kVec], b[kVec];
+    IO<T>::unpack(tp, a);
+    if (q) {
+      IO<T>::unpack(tq, b);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      plain[e] = weight_of(a[e]);
-      const double d = plain[e] - weight_of(b[e]);
-      w[e] = col + e == spike ? 0.0 : (d > 0.0 ? d : 0.0);
+      for (int e = 0; e < kVec; ++e) w[e] = MaxOp()(weight_of(a[e]) - weight_of(b[e]), 0.0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) w[e] = weight_of(a[e]);
+    }
+    if (spike >= col && spike < col + kVec) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) w[e] = col + e == spike ? 0.0 : w[e];
     }
   }
-  // A packet of them that may reach behind `end`, where there are none.
-  __device__ __forceinline__ void weights(int64_t col, int64_t end, double (&w)[kVec],
-                                          double (&plain)[kVec]) const {
-    A a[kVec], b[kVec];
+  __device__ __forceinline__ void weigh(const Piece& at, const u32x4 tp, const u32x4 tq, double (&w)[kVec]) const {
+    weigh(at.col, tp, tq, w);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) a[e] = b[e] = A(0);
-    if (col < end) {
-      const int n = span_of(end - col, kVec);
-      load_span<T>(p + col, n, A(0), a);
-      if (q) load_span<T>(q + col, n, A(0), b);
-    }
-    weigh(col, a, b, w, plain);
+    for (int e = 0; e < kVec; ++e) w[e] = e >= at.dup ? w[e] : 0.0;
   }
 };
-template <typename T>
-__device__ __forceinline__ SampleRow<T> plain_row(const SampleRow<T>& r) {
-  return {r.p, nullptr, -1};
-}
 
-// Inclusive sums over a wavefront's lanes.
+// Sum of a 64-bit value over a wavefront, for every lane, in a fixed order: four steps inside rows
+// of 16 lanes by the data-parallel moves of the vector unit, then the four rows' results. A third of
+// the latency of six shuffles through LDS, which are what short rows wait for.
+template <int kCtrl>
+__device__ __forceinline__ double dpp_add(double v) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), kCtrl, 0xf, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), kCtrl, 0xf, 0xf, false);
+  return v + __builtin_bit_cast(double, static_cast<unsigned long long>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(bits), lane);
+  const unsigned hi = __builtin_amdgcn_readlane(static_cast<int>(bits >> 32), lane);
+  return __builtin_bit_cast(double, static_cast<unsigned long long>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  v = dpp_add<0xB1>(v);   // quad_perm [1,0,3,2]
+  v = dpp_add<0x4E>(v);   // quad_perm [2,3,0,1]
+  v = dpp_add<0x141>(v);  // row_half_mirror
+  v = dpp_add<0x140>(v);  // row_mirror
+  return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
+}
+// Inclusive sums over a wavefront's lanes, by the same moves: within rows of 16 lanes, then the last
+// lane of a row to the next row, then lane 31 to the upper half.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double dpp_scan_step(double v) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), kCtrl, kRows, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), kCtrl, kRows, 0xf, false);
+  return v + __builtin_bit_cast(double, static_cast<unsigned long long>(hi) << 32 | lo);
+}
 __device__ __forceinline__ double wave_scan(double v) {
-  const int lane = threadIdx.x & (kWaveSize - 1);
-#pragma unroll
-  for (int o = 1; o < kWaveSize; o <<= 1) {
-    const double up = __shfl_up(v, o, kWaveSize);
-    if (lane >= o) v += up;
-  }
+  v = dpp_scan_step<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = dpp_scan_step<0x112, 0xf>(v);
+  v = dpp_scan_step<0x114, 0xf>(v);
+  v = dpp_scan_step<0x118, 0xf>(v);
+  v = dpp_scan_step<0x142, 0xa>(v);  // row_bcast 15, to rows 1 and 3
+  v = dpp_scan_step<0x143, 0xc>(v);  // row_bcast 31, to rows 2 and 3
   return v;
 }
 
-// A workgroup of 1024 threads reads a part of a row in steps of 1024 packets and keeps the sum of
-// each wavefront's 64 packets of each step: kMaxSteps * 16 runs in the order of the classes. The
-// run that holds the level is then read once more, out of the L2, by one wavefront.
-constexpr int kMaxSteps = 64;
-constexpr int kRuns = kMaxSteps * kLoopWaves;
+// A run is 64 packets of classes, a wavefront's reading. Workgroups sum the runs of a row in steps of
+// one run per wavefront; whoever picks the class finds the run that holds the level among the
+// sums, and only that run is read again.
 template <typename T>
-constexpr int64_t step_classes() { return static_cast<int64_t>(kLoopThreads) * IO<T>::kVec; }
+constexpr int64_t run_classes() { return static_cast<int64_t>(kWaveSize) * IO<T>::kVec; }
 
-// Sums of the runs of [begin, end), at most kMaxSteps steps, into `runs`; their total, and that of
-// the target alone, for every thread. Holds barriers; `runs` and `slots` may be read behind it.
-struct Totals {
-  double weight, plain;
-};
-template <typename T>
-__device__ __forceinline__ Totals sum_runs(const SampleRow<T>& row, int64_t begin, int64_t end,
-                                           double* runs, double (*slots)[kLoopWaves]) {
-  using A = typename IO<T>::Acc;
+// Sums the runs of [begin, end): f(run, sum) is called by every lane of the wavefront that read it.
+// `kWaves` wavefronts take runs in turn, kAtOnce of them requested before the first is summed; the
+// last step may reach runs behind the end, of sum 0.
+template <int kWaves, int kAtOnce, typename T, typename F>
+__device__ __forceinline__ void sum_runs(const SampleRow<T>& row, const int64_t begin, const int64_t end,
+                                         F&& f) {
   constexpr int kVec = IO<T>::kVec;
-  // steps requested before the first is summed: 64 and 128 KB per workgroup; with four of eight
-  // classes a thread spills
-  constexpr int kAtOnce = kVec == 8 ? 2 : 4;
-  constexpr int64_t kStep = step_classes<T>();
-  const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
-  double weight = 0.0, plain = 0.0;
-  int step = 0;
-  auto take = [&](int at_step, const double(&w)[kVec], const double(&pl)[kVec]) {
-    double sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      sum += w[e];
-      plain += pl[e];
-    }
-    sum = wave_allreduce(sum, SumOp());
-    weight += sum;
-    if (lane == 0) runs[at_step * kLoopWaves + wave] = sum;
-  };
-  int64_t at = begin + static_cast<int64_t>(threadIdx.x) * kVec;
-  for (; begin + kAtOnce * kStep <= end; begin += kAtOnce * kStep, at += kAtOnce * kStep, step += kAtOnce) {
+  constexpr int64_t kStep = kWaves * run_classes<T>();
+  int64_t run = threadIdx.x / kWaveSize;
+  for (int64_t at = begin + static_cast<int64_t>(threadIdx.x) * kVec, base = begin; base < end;
+       base += kAtOnce * kStep, at += kAtOnce * kStep) {
     u32x4 rp[kAtOnce], rq[kAtOnce];
+    double sum[kAtOnce];
+    if (base + kAtOnce * kStep <= end) {
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      rp[k] = load_packet_unaligned(row.p + at + k * kStep);
-      if (row.q) rq[k] = load_packet_unaligned(row.q + at + k * kStep);
-    }
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      A a[kVec], b[kVec];
-      IO<T>::unpack(rp[k], a);
-      if (row.q) {
-        IO<T>::unpack(rq[k], b);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) b[e] = A(0);
+      for (int k = 0; k < kAtOnce; ++k) {
+        rp[k] = load_packet_once(row.p + at + k * kStep);
+        if (row.q) rq[k] = load_packet_once(row.q + at + k * kStep);
       }
-      double w[kVec], pl[kVec];
-      row.weigh(at + k * kStep, a, b, w, pl);
-      take(step + k, w, pl);
-      __builtin_amdgcn_sched_barrier(0);  // one packet's 64-bit values at a time
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        double w[kVec];
+        row.weigh(at + k * kStep, rp[k], rq[k], w);
+        sum[k] = w[0];
+#pragma unroll
+        for (int e = 1; e < kVec; ++e) sum[k] += w[e];
+        __builtin_amdgcn_sched_barrier(0);  // one packet's 64-bit values at a time
+      }
+    } else {
+      typename SampleRow<T>::Piece piece[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        piece[k] = row.piece(at + k * kStep, end);
+        rp[k] = row.packet(row.p, piece[k], end);
+        if (row.q) rq[k] = row.packet(row.q, piece[k], end);
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        double w[kVec];
+        row.weigh(piece[k], rp[k], rq[k], w);
+        sum[k] = w[0];
+#pragma unroll
+        for (int e = 1; e < kVec; ++e) sum[k] += w[e];
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) sum[k] = wave_sum(sum[k]);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k, run += kWaves) f(run, sum[k]);
   }
-  for (; begin < end; begin += kStep, at += kStep, ++step) {
-    double w[kVec], pl[kVec];
-    row.weights(at, end, w, pl);
-    take(step, w, pl);
-  }
-  weight = block_allreduce<kLoopWaves>(lane == 0 ? weight : 0.0, SumOp(), slots[0]);
-  return {weight, block_allreduce<kLoopWaves>(plain, SumOp(), slots[1])};
 }
 
-// The lowest class of [begin, end) whose running sum, from `before` at begin, exceeds `level`; the
-// last class of non-zero weight where rounding leaves none; -1 where there is no weight. Called
-// by the first wavefront, behind sum_runs of the same part.
-template <typename T>
-__device__ __forceinline__ int64_t pick_class(const SampleRow<T>& row, int64_t begin, int64_t end,
-                                              double before, const double level, const double* runs) {
-  constexpr int kVec = IO<T>::kVec;
-  const int lane = threadIdx.x & (kWaveSize - 1);
-  const int64_t steps = ceil_div_device(end - begin, step_classes<T>());
-  const int count = static_cast<int>(steps) * kLoopWaves;
-  // the first run behind which the sum exceeds the level, else the last one with weight
-  int chosen = -1, last = -1;
-  double at = before, chosen_before = before, last_before = before;
-  for (int first = 0; first < count && chosen < 0; first += kWaveSize) {
-    const double mine = first + lane < count ? runs[first + lane] : 0.0;
-    const double upto = wave_scan(mine);
-    const unsigned long long hit = __ballot(mine > 0.0 && at + upto > level);
-    const unsigned long long any = __ballot(mine > 0.0);
-    const int l = hit ? __builtin_ctzll(hit) : (any ? 63 - __builtin_clzll(any) : 0);
-    const double from = at + __shfl(upto - mine, l, kWaveSize);
-    if (hit) chosen = first + l, chosen_before = from;
-    else if (any) last = first + l, last_before = from;
-    at += __shfl(upto, kWaveSize - 1, kWaveSize);
-  }
-  if (chosen < 0) {
-    if (last < 0) return -1;
-    chosen = last, chosen_before = last_before;
-  }
-  const int64_t col = begin + (static_cast<int64_t>(chosen) * kWaveSize + lane) * kVec;
-  double w[kVec], plain[kVec];
-  row.weights(col, end, w, plain);
-  double mine = 0.0;
-  int64_t held = -1;
+// Picks the class by the sums of a row's `count` runs: the lowest one whose running sum exceeds
+// u * total; the last class of non-zero weight where rounding (or u >= 1) leaves none; -1 where
+// there is no weight. A residual without weight gives way to the target, whose runs are summed
+// here and take the others' place. By a workgroup of kWaves wavefronts, each thread of which
+// takes a stretch of the runs; the class is returned to the first wavefront.
+template <int kWaves, typename T>
+__device__ __forceinline__ int64_t pick_class(SampleRow<T> row, const int64_t C, const int64_t count,
+                                              double* runs, const float u) {
+  constexpr int kVec = IO<T>::kVec, kThreads = kWaves * kWaveSize;
+  __shared__ double waves[kWaves];
+  __shared__ int64_t hits[kWaves], lasts[kWaves];
+  __shared__ double hit_before[kWaves], last_before[kWaves];
+  const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
+  const int64_t stretch = ceil_div_device(count, kThreads);
+  const int64_t from = threadIdx.x * stretch < count ? threadIdx.x * stretch : count;
+  const int64_t to = from + stretch < count ? from + stretch : count;
+  double mine, upto, total;
+  for (;;) {
+    mine = 0.0;
+    for (int64_t r = from; r < to; ++r) mine += runs[r];
+    upto = wave_scan(mine);
+    if (lane == kWaveSize - 1) waves[wave] = upto;
+    __syncthreads();
+    total = 0.0;
+    double before = 0.0;
 #pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    mine += w[e];
-    if (w[e] > 0.0) held = col + e;
+    for (int i = 0; i < kWaves; ++i) {
+      if (i == wave) before = total;
+      total += waves[i];
+    }
+    upto += before;
+    if (total > 0.0 || (!row.q && row.spike < 0)) break;
+    row.q = nullptr, row.spike = -1;
+    __syncthreads();  // every thread has read the sums
+    sum_runs<kWaves, 2>(row, 0, C, [&](int64_t run, double sum) {
+      if (lane == 0 && run < count) runs[run] = sum;
+    });
+    __syncthreads();
   }
-  double run = chosen_before + (wave_scan(mine) - mine);
-  int64_t found = -1;
+  const double level = u > 0.f ? static_cast<double>(u) * total : 0.0;
+  // the first run of the stretch behind which the sum exceeds the level, and the last with weight
+  int64_t hit = -1, last = -1;
+  double run = upto - mine, at_hit = 0.0, at_last = 0.0;
+  if (mine > 0.0) {
+    for (int64_t r = from; r < to; ++r) {
+      const double w = runs[r];
+      if (w > 0.0) {
+        if (hit < 0 && run + w > level) hit = r, at_hit = run;
+        last = r, at_last = run;
+      }
+      run += w;
+    }
+  }
+  const unsigned long long hit_lanes = __ballot(hit >= 0), last_lanes = __ballot(last >= 0);
+  const int h = hit_lanes ? __builtin_ctzll(hit_lanes) : 0;
+  const int l = last_lanes ? 63 - __builtin_clzll(last_lanes) : 0;
+  if (lane == h) hits[wave] = hit, hit_before[wave] = at_hit;
+  if (lane == l) lasts[wave] = last, last_before[wave] = at_last;
+  __syncthreads();
+  if (wave != 0) return -1;
+  int64_t chosen = -1;
+  double before = 0.0;
+#pragma unroll
+  for (int i = kWaves - 1; i >= 0; --i)
+    if (hits[i] >= 0) chosen = hits[i], before = hit_before[i];
+  if (chosen < 0) {
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i)
+      if (lasts[i] >= 0) chosen = lasts[i], before = last_before[i];
+    if (chosen < 0) return -1;
+  }
+  const typename SampleRow<T>::Piece piece = row.piece(chosen * run_classes<T>() + lane * kVec, C);
+  const int64_t col = piece.col;
+  double w[kVec];
+  const u32x4 none = {0u, 0u, 0u, 0u};
+  row.weigh(piece, row.packet(row.p, piece, C), row.q ? row.packet(row.q, piece, C) : none, w);
+  double sum = w[0];
+  int64_t held = -1, found = -1;
+#pragma unroll
+  for (int e = 1; e < kVec; ++e) sum += w[e];
+  run = before + (wave_scan(sum) - sum);
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
     run += w[e];
-    if (found < 0 && w[e] > 0.0 && run > level) found = col + e;
+    if (w[e] > 0.0) {
+      held = col + e;
+      if (found < 0 && run > level) found = col + e;
+    }
   }
-  const unsigned long long hit = __ballot(found >= 0);
-  if (hit) return __shfl(found, __builtin_ctzll(hit), kWaveSize);
-  const unsigned long long any = __ballot(held >= 0);
-  return any ? __shfl(held, 63 - __builtin_clzll(any), kWaveSize) : -1;
+  const unsigned long long found_lanes = __ballot(found >= 0), held_lanes = __ballot(held >= 0);
+  if (found_lanes) return __shfl(found, __builtin_ctzll(found_lanes), kWaveSize);
+  return held_lanes ? __shfl(held, 63 - __builtin_clzll(held_lanes), kWaveSize) : -1;
 }
 
-template <typename IndexT>
-__device__ __forceinline__ int64_t length_of(const IndexT* lengths, int64_t b, int64_t K) {
-  if (!lengths) return K;
-  const int64_t len = static_cast<int64_t>(lengths[b]);
-  return len < 0 ? 0 : (len > K ? K : len);
-}
 template <typename T, typename IndexT>
-__device__ __forceinline__ SampleRow<T> sample_row(int64_t b, int64_t K, int64_t C, int64_t n, int64_t len,
+__device__ __forceinline__ SampleRow<T> sample_row(int64_t b, int64_t K, int64_t C, const Verdict& v,
                                                    const T* target, const T* draft, const IndexT* drafted) {
-  SampleRow<T> row = {target + (b * (K + 1) + n) * C, nullptr, -1};
-  if (n < len) {
-    if (draft) row.q = draft + (b * K + n) * C;
-    else row.spike = static_cast<int64_t>(drafted[b * K + n]);
+  SampleRow<T> row = {target + (b * (K + 1) + v.n) * C, nullptr, -1};
+  if (v.n < v.len) {
+    if (draft) row.q = draft + (b * K + v.n) * C;
+    else row.spike = static_cast<int64_t>(drafted[b * K + v.n]);
   }
   return row;
 }
-__device__ __forceinline__ double level_of(float u, double total) {
-  return u > 0.f ? static_cast<double>(u) * total : 0.0;
-}
 
-// A sequence by one workgroup: rows of one part.
+// A sequence by one workgroup, the sums of its runs in LDS: one launch.
+constexpr int kRowsWaves = 16, kMaxRuns = 1024;
 template <typename T, typename IndexT>
-__global__ __launch_bounds__(kLoopThreads) void draft_verify_rows(
+__global__ __launch_bounds__(kRowsWaves * kWaveSize) void draft_verify_rows(
     const int64_t B, const int64_t K, const int64_t C, const T* __restrict__ target,
     const T* __restrict__ draft, const IndexT* __restrict__ drafted, const IndexT* __restrict__ lengths,
     const float* __restrict__ u_accept, const float* __restrict__ u_sample, IndexT* __restrict__ tokens,
     IndexT* __restrict__ accepted) {
-  __shared__ double runs[kRuns];
-  __shared__ double slots[2][kLoopWaves];
-  __shared__ int64_t count;
+  __shared__ double runs[kMaxRuns];
+  __shared__ Verdict verdict;
+  const int lane = threadIdx.x & (kWaveSize - 1);
   for (int64_t b = blockIdx.x; b < B; b += gridDim.x) {
-    const int64_t len = length_of(lengths, b, K);
+    const float u = u_sample[b];
     if (threadIdx.x < kWaveSize) {
-      const int64_t n = count_accepted(b, K, C, len, target, draft, drafted, u_accept);
-      if (threadIdx.x == 0) count = n;
+      const Verdict v = judge(b, K, C, target, draft, drafted, lengths, u_accept);
+      if (threadIdx.x == 0) verdict = v;
     }
     __syncthreads();
-    const int64_t n = count;
-    SampleRow<T> row = sample_row(b, K, C, n, len, target, draft, drafted);
-    double total = sum_runs(row, 0, C, runs, slots).weight;
-    if (!(total > 0.0) && (row.q || row.spike >= 0)) {  // a residual without weight gives way to the target
-      __syncthreads();
-      row = plain_row(row);
-      total = sum_runs(row, 0, C, runs, slots).weight;
-    }
-    if (threadIdx.x < kWaveSize) {
-      const int64_t token = pick_class(row, 0, C, 0.0, level_of(u_sample[b], total), runs);
-      if (threadIdx.x == 0) {
-        tokens[b * (K + 1) + n] = static_cast<IndexT>(token);
-        accepted[b] = static_cast<IndexT>(n);
-      }
-    }
-    for (int64_t i = threadIdx.x; i <= K; i += kLoopThreads) {
-      if (i != n) tokens[b * (K + 1) + i] = i < n ? drafted[b * K + i] : IndexT(-1);
-    }
-    __syncthreads();  // runs, slots and count are reused by the next sequence
-  }
-}
-
-// Rows cut into parts, for long rows of few sequences: first the totals of every part, of the
-// residual and of the target itself, then a workgroup per sequence finds the part that holds the
-// level and does as above with it.
-template <typename T, typename IndexT>
-__global__ __launch_bounds__(kLoopThreads) void draft_verify_parts(
-    const int64_t B, const int64_t K, const int64_t C, const int64_t part, const T* __restrict__ target,
-    const T* __restrict__ draft, const IndexT* __restrict__ drafted, const IndexT* __restrict__ lengths,
-    const float* __restrict__ u_accept, IndexT* __restrict__ accepted, Totals* __restrict__ totals) {
-  __shared__ double runs[kRuns];
-  __shared__ double slots[2][kLoopWaves];
-  __shared__ int64_t count;
-  const int64_t begin = blockIdx.y * part;
-  const int64_t end = begin + part < C ? begin + part : C;
-  for (int64_t b = blockIdx.x; b < B; b += gridDim.x) {
-    const int64_t len = length_of(lengths, b, K);
-    if (threadIdx.x < kWaveSize) {
-      const int64_t n = count_accepted(b, K, C, len, target, draft, drafted, u_accept);
-      if (threadIdx.x == 0) count = n;
-    }
+    const Verdict v = verdict;
+    const SampleRow<T> row = sample_row(b, K, C, v, target, draft, drafted);
+    sum_runs<kRowsWaves, 2>(row, 0, C, [&](int64_t run, double sum) {
+      if (lane == 0 && run < kMaxRuns) runs[run] = sum;
+    });
     __syncthreads();
-    const int64_t n = count;
-    const SampleRow<T> row = sample_row(b, K, C, n, len, target, draft, drafted);
-    const Totals total = sum_runs(row, begin, end, runs, slots);
+    const int64_t token = pick_class<kRowsWaves>(row, C, ceil_div_device(C, run_classes<T>()), runs, u);
     if (threadIdx.x == 0) {
-      totals[b * gridDim.y + blockIdx.y] = total;
-      if (blockIdx.y == 0) accepted[b] = static_cast<IndexT>(n);
+      tokens[b * (K + 1) + v.n] = static_cast<IndexT>(token);
+      accepted[b] = static_cast<IndexT>(v.n);
     }
-    __syncthreads();
-  }
-}
-template <typename T, typename IndexT>
-__global__ __launch_bounds__(kLoopThreads) void draft_verify_join(
-    const int64_t B, const int64_t K, const int64_t C, const int64_t part, const int parts,
-    const T* __restrict__ target, const T* __restrict__ draft, const IndexT* __restrict__ drafted,
-    const IndexT* __restrict__ lengths, const float* __restrict__ u_sample, IndexT* __restrict__ tokens,
-    const IndexT* __restrict__ accepted, const Totals* __restrict__ totals) {
-  __shared__ double runs[kRuns];
-  __shared__ double slots[2][kLoopWaves];
-  for (int64_t b = blockIdx.x; b < B; b += gridDim.x) {
-    const int64_t len = length_of(lengths, b, K);
-    const int64_t n = static_cast<int64_t>(accepted[b]);
-    SampleRow<T> row = sample_row(b, K, C, n, len, target, draft, drafted);
-    const Totals* sums = totals + b * parts;
-    double total = 0.0;
-    for (int i = 0; i < parts; ++i) total += sums[i].weight;
-    const bool plain = !(total > 0.0);  // a residual without weight gives way to the target
-    if (plain) {
-      row = plain_row(row);
-      total = 0.0;
-      for (int i = 0; i < parts; ++i) total += sums[i].plain;
+    for (int64_t i = threadIdx.x; i <= K; i += kRowsWaves * kWaveSize) {
+      if (i != v.n) tokens[b * (K + 1) + i] = i < v.n ? drafted[b * K + i] : IndexT(-1);
     }
-    const double level = level_of(u_sample[b], total);
-    // the part that holds the level, else the last one with weight
-    int chosen = -1, last = 0;
-    double at = 0.0, before = 0.0, last_before = 0.0;
-    for (int i = 0; i < parts && chosen < 0; ++i) {
-      const double sum = plain ? sums[i].plain : sums[i].weight;
-      if (sum > 0.0) {
-        last = i, last_before = at;
-        if (at + sum > level) chosen = i, before = at;
-      }
-      at += sum;
-    }
-    if (chosen < 0) chosen = last, before = last_before;
-    const int64_t begin = chosen * part;
-    const int64_t end = begin + part < C ? begin + part : C;
-    sum_runs(row, begin, end, runs, slots);
-    int64_t token = -1;
-    if (threadIdx.x < kWaveSize) token = pick_class(row, begin, end, before, level, runs);
-    if (threadIdx.x == 0) tokens[b * (K + 1) + n] = static_cast<IndexT>(token);
-    for (int64_t i = threadIdx.x; i <= K; i += kLoopThreads) {
-      if (i != n) tokens[b * (K + 1) + i] = i < n ? drafted[b * K + i] : IndexT(-1);
-    }
-    __syncthreads();
+    __syncthreads();  // the LDS is reused by the next sequence
   }
 }
 
-// Parts of a row: one where a workgroup's runs hold it and there are sequences enough to fill the
-// device, or the row is short; else parts of at least four steps (the loads that a workgroup has
-// in flight at once), twice as many workgroups as compute units at most.
+// Long rows: workgroups of four wavefronts sum the runs of a part of a row each, and a second launch
+// picks the classes, a workgroup per sequence.
+constexpr int kPartWaves = 4;
+template <typename T, typename IndexT>
+__global__ __launch_bounds__(kPartWaves * kWaveSize) void draft_verify_runs(
+    const int64_t B, const int64_t K, const int64_t C, const uint32_t parts, const int64_t part_runs,
+    const int64_t row_runs, const T* __restrict__ target, const T* __restrict__ draft,
+    const IndexT* __restrict__ drafted, const IndexT* __restrict__ lengths,
+    const float* __restrict__ u_accept, IndexT* __restrict__ accepted, double* __restrict__ sums) {
+  __shared__ Verdict verdict;
+  const int lane = threadIdx.x & (kWaveSize - 1);
+  for (int64_t item = blockIdx.x; item < B * parts; item += gridDim.x) {
+    const int64_t b = item / parts, part = item - b * parts;
+    if (threadIdx.x < kWaveSize) {
+      const Verdict v = judge(b, K, C, target, draft, drafted, lengths, u_accept);
+      if (threadIdx.x == 0) {
+        verdict = v;
+        if (part == 0) accepted[b] = static_cast<IndexT>(v.n);
+      }
+    }
+    __syncthreads();
+    const SampleRow<T> row = sample_row(b, K, C, verdict, target, draft, drafted);
+    const int64_t first = part * part_runs, last = first + part_runs < row_runs ? first + part_runs : row_runs;
+    const int64_t begin = first * run_classes<T>();
+    const int64_t end = last * run_classes<T>() < C ? last * run_classes<T>() : C;
+    double* out = sums + b * row_runs + first;
+    sum_runs<kPartWaves, IO<T>::kVec == 8 ? 2 : 4>(row, begin, end, [&](int64_t run, double sum) {
+      if (lane == 0 && first + run < last) out[run] = sum;
+    });
+    __syncthreads();  // the verdict is overwritten by the next item's
+  }
+}
+template <typename T, typename IndexT>
+__global__ __launch_bounds__(kPartWaves * kWaveSize) void draft_verify_pick(
+    const int64_t B, const int64_t K, const int64_t C, const int64_t row_runs, const T* __restrict__ target,
+    const T* __restrict__ draft, const IndexT* __restrict__ drafted, const IndexT* __restrict__ lengths,
+    const float* __restrict__ u_sample, IndexT* __restrict__ tokens, const IndexT* __restrict__ accepted,
+    double* __restrict__ sums) {
+  for (int64_t b = blockIdx.x; b < B; b += gridDim.x) {
+    const Verdict v = {static_cast<int64_t>(accepted[b]), length_of(lengths, b, K)};
+    const SampleRow<T> row = sample_row(b, K, C, v, target, draft, drafted);
+    const int64_t token = pick_class<kPartWaves>(row, C, row_runs, sums + b * row_runs, u_sample[b]);
+    if (threadIdx.x == 0) tokens[b * (K + 1) + v.n] = static_cast<IndexT>(token);
+    for (int64_t i = threadIdx.x; i <= K; i += kPartWaves * kWaveSize) {
+      if (i != v.n) tokens[b * (K + 1) + i] = i < v.n ? drafted[b * K + i] : IndexT(-1);
+    }
+    __syncthreads();  // the LDS of pick_class is reused by the next sequence
+  }
+}
+
+// One workgroup takes a row whole up to 32768 classes, where one compute unit needs as long for them
+// (fp32 [1, 5, 32000]: 9.7 us) as a second launch costs, and where there are two sequences and
+// more per compute unit. Other rows are cut into parts of 4 to 64 runs per wavefront, as many as 16
+// workgroups per compute unit make of them: short streams, of neighbouring workgroups, lie close
+// together in memory (fp32 [192, 6, 131072]: 47 us with 5 workgroups per compute unit, 38 with 16,
+// 37 with 48).
 struct PartPlan {
-  int64_t parts, classes;  // per row, per part
+  int64_t parts, part_runs, row_runs;  // parts = 0: whole rows
 };
 template <typename T>
 PartPlan plan_parts(int64_t B, int64_t C) {
-  const int64_t steps = ceil_div(C, step_classes<T>());
-  const int64_t fewest = ceil_div(steps, kMaxSteps);
-  int64_t parts = ceil_div(static_cast<int64_t>(num_cus()) * 2, B > 0 ? B : 1);
-  if (parts > steps / 4) parts = steps / 4;
-  if (B * 2 > num_cus() || parts < 1) parts = 1;
-  if (parts < fewest) parts = fewest;
-  const int64_t each = ceil_div(steps, parts);
-  return {ceil_div(steps, each), each * step_classes<T>()};
+  const int64_t runs = ceil_div(C, run_classes<T>());
+  if (C <= 32768 || (B >= 2 * num_cus() && runs <= kMaxRuns)) return {0, runs, runs};
+  int64_t parts = static_cast<int64_t>(num_cus()) * 16 / B;
+  const int64_t most = ceil_div(runs, kPartWaves * 4), fewest = ceil_div(runs, kPartWaves * 64);
+  parts = parts > most ? most : (parts < fewest ? fewest : parts);
+  const int64_t each = ceil_div(ceil_div(runs, parts), kPartWaves) * kPartWaves;
+  return {ceil_div(runs, each), each, runs};
 }
 
 template <typename T, typename IndexT>
@@ -386,18 +448,19 @@ int launch_verify(int64_t B, int64_t K, int64_t C, const void* target, const voi
   IndexT* op = static_cast<IndexT*>(tokens);
   IndexT* ap = static_cast<IndexT*>(accepted);
   const PartPlan plan = plan_parts<T>(B, C);
-  const unsigned grid = row_grid(B, 1);
-  if (plan.parts == 1) {
-    hipLaunchKernelGGL((draft_verify_rows<T, IndexT>), dim3(grid), dim3(kLoopThreads), 0, stream, B, K, C,
-                       tp, qp, dp, lp, ua, us, op, ap);
+  if (plan.parts == 0) {
+    hipLaunchKernelGGL((draft_verify_rows<T, IndexT>), dim3(row_grid(B, 1)), dim3(kRowsWaves * kWaveSize), 0,
+                       stream, B, K, C, tp, qp, dp, lp, ua, us, op, ap);
   } else {
-    Totals* totals = static_cast<Totals*>(scratch);
-    if (!totals || scratch_bytes < static_cast<size_t>(B * plan.parts) * sizeof(Totals))
+    double* sums = static_cast<double*>(scratch);
+    if (!sums || scratch_bytes < static_cast<size_t>(B * plan.row_runs) * sizeof(double))
       return DRAGON_HIP_ESCRATCH;
-    hipLaunchKernelGGL((draft_verify_parts<T, IndexT>), dim3(grid, static_cast<unsigned>(plan.parts)),
-                       dim3(kLoopThreads), 0, stream, B, K, C, plan.classes, tp, qp, dp, lp, ua, ap, totals);
-    hipLaunchKernelGGL((draft_verify_join<T, IndexT>), dim3(grid), dim3(kLoopThreads), 0, stream, B, K, C,
-                       plan.classes, static_cast<int>(plan.parts), tp, qp, dp, lp, us, op, ap, totals);
+    const dim3 block(kPartWaves * kWaveSize);
+    hipLaunchKernelGGL((draft_verify_runs<T, IndexT>), dim3(row_grid(B * plan.parts, 1)), block, 0, stream,
+                       B, K, C, static_cast<uint32_t>(plan.parts), plan.part_runs, plan.row_runs, tp, qp, dp,
+                       lp, ua, ap, sums);
+    hipLaunchKernelGGL((draft_verify_pick<T, IndexT>), dim3(row_grid(B, 1)), block, 0, stream, B, K, C,
+                       plan.row_runs, tp, qp, dp, lp, us, op, ap, sums);
   }
   return status_of_launch();
 }
@@ -417,7 +480,7 @@ int launch_verify_index(int index_dtype, int64_t B, int64_t K, int64_t C, const 
 template <typename T>
 size_t verify_scratch_bytes(int64_t B, int64_t C) {
   const PartPlan plan = plan_parts<T>(B, C);
-  return plan.parts == 1 ? 0 : static_cast<size_t>(B * plan.parts) * sizeof(Totals);
+  return plan.parts == 0 ? 0 : static_cast<size_t>(B * plan.row_runs) * sizeof(double);
 }
 
 } // namespace
