@@ -363,19 +363,27 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
   else DRAGON_HIP_RMS_SWITCH_2(packets, LAUNCH)
 constexpr int64_t kMaxTilePackets = 4096;
 
+// Workgroups that walk the rows: eight wavefronts per compute unit, each with its next row's packets
+// in flight. Measured with four, eight and as many wavefronts as fit (sixteen to
+// twenty-four): bf16 [8192, 8192] with a residual 109 us at four, 91 at eight, 92 at twenty-four, 99
+// with a workgroup per row; its gradient at [8192, 4096] 49 us at eight, 53 at sixteen, 58 at
+// thirty-two. More streams at a time are further apart in memory, and leave more partial sums.
+inline int64_t rms_grid(int threads) {
+  return static_cast<int64_t>(num_cus()) * (threads < 512 ? 512 / threads : 1);
+}
+
 template <typename T, int kTPR, int kVPT, bool kRagged, bool kResidual, int kOut>
 int launch_rms_tile(int64_t N, int64_t C, float eps, const void* x, const void* residual,
                     const void* gamma, void* h, void* rsig, void* y, int64_t group, int64_t groups,
                     void* q, void* scale, hipStream_t stream) {
   using A = typename IO<T>::Acc;
-  auto kernel = rms_norm_rows<T, kTPR, kVPT, kRagged, kResidual, kOut>;
   constexpr int kThreads = tile_threads(kTPR);
   const int64_t want = ceil_div(N, kThreads / kTPR);
-  const int64_t resident = resident_grid(kernel, kThreads, 0);
+  const int64_t most = rms_grid(kThreads);
   note_number("threads_per_row", kTPR);
   note_number("packets", kVPT);
   hipLaunchKernelGGL((rms_norm_rows<T, kTPR, kVPT, kRagged, kResidual, kOut>),
-                     dim3(static_cast<unsigned>(want < resident ? want : resident)), dim3(kThreads), 0,
+                     dim3(static_cast<unsigned>(want < most ? want : most)), dim3(kThreads), 0,
                      stream, N, static_cast<int>(C), A(eps), static_cast<const T*>(x),
                      static_cast<const T*>(residual), static_cast<const A*>(gamma), static_cast<T*>(h),
                      static_cast<A*>(rsig), static_cast<T*>(y), static_cast<int>(group),
@@ -539,7 +547,7 @@ __global__ __launch_bounds__(kColThreads) void rms_norm_grad_cols(
 // of a workgroup add theirs in LDS, in order, and each workgroup leaves one row of partial sums.
 constexpr int grad_threads(int tpr) { return tpr <= 512 ? 512 : 1024; }
 template <typename T, int kTPR, int kVPT, bool kRagged, bool kThrough>
-__global__ __launch_bounds__(grad_threads(kTPR), 4) void rms_norm_grad_rows(
+__global__ __launch_bounds__(grad_threads(kTPR)) void rms_norm_grad_rows(
     const int64_t N, const int C, const T* h, const typename IO<T>::Acc* rsig,
     const typename IO<T>::Acc* gamma, const T* dy, const T* dh, typename IO<T>::Acc* partial, T* dx) {
   using A = typename IO<T>::Acc;
@@ -714,8 +722,7 @@ inline GradCols plan_grad_cols(int64_t N, int64_t C, int vec) {
   return p;
 }
 
-// Rows that the register tiles hold: their workgroups (two of 512 threads or one of 1024 per
-// compute unit, by registers), each of which leaves a row of partial sums.
+// Rows that the register tiles hold: their workgroups, each of which leaves a row of partial sums.
 // Four packets of 16-bit elements per thread (three tensors' and as many sums) do not fit the
 // registers of 1024 threads.
 template <typename T>
@@ -731,7 +738,7 @@ int64_t grad_grid(int64_t N, int64_t C) {
 #undef TAKE
   const int threads = grad_threads(tpr);
   const int64_t want = ceil_div(N, threads / tpr);
-  const int64_t most = static_cast<int64_t>(num_cus()) * (threads == 512 ? 2 : 1);
+  const int64_t most = rms_grid(threads);
   return want < most ? want : most;
 }
 
