@@ -306,80 +306,101 @@ def broadcast_loss_grad(N, S, C, dl, dx):
 
 _BYTE_DTYPES = (torch.uint8, torch.float8_e4m3fn)
 _ACC_DTYPES = {0: torch.float32, 1: torch.float32, 2: torch.float32, 3: torch.float64}
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
-class _Args:
-    """Checks the tensors of one call against its sizes and gives their addresses: all on the
-    current device, contiguous, of the type asked for and of at least so many elements."""
+def _refuse(t, device, numel, dtype):
+    """Says what is wrong with an argument that _arg did not take."""
+    if t is None:
+        raise ValueError("a tensor is missing")
+    if t.get_device() != device:
+        raise ValueError("kernel arguments must live in the memory of the current device")
+    if not t.is_contiguous():
+        raise ValueError("kernel arguments must be contiguous")
+    if t.numel() < numel:
+        raise ValueError("a tensor of %d elements where the sizes ask for %d" % (t.numel(), numel))
+    raise TypeError("a tensor of %s where %s is expected" % (t.dtype, dtype))
 
-    def __init__(self):
-        self.device = torch.cuda.current_device()
 
-    def __call__(self, t, numel, dtype, optional=False):
-        if t is None:
-            if optional or numel == 0:
-                return None
-            raise ValueError("a tensor is missing")
-        if t.get_device() != self.device:
-            raise ValueError("kernel arguments must live in the memory of the current device")
-        if not t.is_contiguous():
-            raise ValueError("kernel arguments must be contiguous")
-        if t.dtype is not dtype and not (type(dtype) is tuple and t.dtype in dtype):
-            raise TypeError("a tensor of %s where %s is expected" % (t.dtype, dtype))
-        if t.numel() < numel:
-            raise ValueError("a tensor of %d elements where the sizes ask for %d" % (t.numel(), numel))
-        return t.data_ptr()
+def _arg(t, device, numel, dtype):
+    """The address of a tensor that a call reads or writes ``numel`` elements of: contiguous, of the
+    type asked for, on the current device. A tensor of no elements may be missing."""
+    if t is None and numel == 0:
+        return None
+    if (t is None or t.dtype is not dtype or t.numel() < numel or t.get_device() != device or
+            not t.is_contiguous()):
+        _refuse(t, device, numel, dtype)
+    return t.data_ptr()
 
-    def stream(self):
-        return torch._C._cuda_getCurrentRawStream(self.device)
 
-    def scratch(self, nbytes):
-        """Scratch for the current stream. While a graph is being captured it comes from that
-        graph's own memory, so that graphs share none and a later, larger call cannot free it."""
-        if nbytes == 0:
-            return None
-        if torch.cuda.is_current_stream_capturing():
-            return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        return workspace(nbytes, torch.device("cuda", self.device))
+def _opt(t, device, numel, dtype):
+    """The same for a tensor that may be None."""
+    return None if t is None else _arg(t, device, numel, dtype)
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _scratch_for(device, nbytes):
+    """Scratch of a call on the current stream. While a graph is being captured it comes from that
+    graph's own memory, so that graphs share none and a later, larger call cannot free it."""
+    if nbytes == 0:
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    buf = _scratch.get((device, _raw_stream(device)))
+    if buf is None or buf.numel() < nbytes:
+        buf = workspace(nbytes, torch.device("cuda", device))
+    return buf
 
 
 def _sizes(*sizes):
-    if min(sizes) < 0:
-        raise ValueError("negative size in %s" % (sizes,))
+    for n in sizes:
+        if n < 0:
+            raise ValueError("negative size in %s" % (sizes,))
+
+
+def _run(name, *args):
+    status = getattr(_lib.lib(), name)(*args)
+    if status:
+        _lib.check(name, status)
 
 
 def rms_norm(N, C, epsilon, x, residual, gamma, h, rsig, y):
     """h = x + residual, y = h / sqrt(mean(h^2) + epsilon) * gamma over rows of C. residual, h and
     rsig may be None; y and h may be the tensors x or residual themselves."""
     _sizes(N, C)
-    a, tag, n = _Args(), dtype_tag(x), N * C
-    acc, dt = _ACC_DTYPES[tag], x.dtype
-    _call("dragon_hip_rms_norm", tag, N, C, epsilon, a(x, n, dt), a(residual, n, dt, True),
-          a(gamma, C, acc), a(h, n, dt, True), a(rsig, N, acc, True), a(y, n, dt), a.stream())
+    dev, tag, n, dt = _current_device(), dtype_tag(x), N * C, x.dtype
+    acc = _ACC_DTYPES[tag]
+    _run("dragon_hip_rms_norm", tag, N, C, epsilon, _arg(x, dev, n, dt), _opt(residual, dev, n, dt),
+         _arg(gamma, dev, C, acc), _opt(h, dev, n, dt), _opt(rsig, dev, N, acc), _arg(y, dev, n, dt),
+         _raw_stream(dev))
 
 
 def rms_norm_quant(N, C, group, epsilon, x, residual, gamma, h, rsig, q, scale):
     """rms_norm with y as e4m3 codes (uint8 or float8_e4m3fn) and a float32 scale per group of
     columns (32, 64, 128 or 256; 0: per row): y = q * scale."""
     _sizes(N, C, group)
-    a, tag, n = _Args(), dtype_tag(x), N * C
-    dt, groups = x.dtype, -(-C // group) if group else 1
-    _call("dragon_hip_rms_norm_quant", tag, N, C, group, epsilon, a(x, n, dt), a(residual, n, dt, True),
-          a(gamma, C, _ACC_DTYPES[tag]), a(h, n, dt, True), a(rsig, N, _ACC_DTYPES[tag], True),
-          a(q, n, _BYTE_DTYPES), a(scale, N * groups, torch.float32), a.stream())
+    dev, tag, n, dt = _current_device(), dtype_tag(x), N * C, x.dtype
+    acc, groups = _ACC_DTYPES[tag], -(-C // group) if group else 1
+    code = q.dtype if q is not None and q.dtype in _BYTE_DTYPES else torch.uint8
+    _run("dragon_hip_rms_norm_quant", tag, N, C, group, epsilon, _arg(x, dev, n, dt),
+         _opt(residual, dev, n, dt), _arg(gamma, dev, C, acc), _opt(h, dev, n, dt), _opt(rsig, dev, N, acc),
+         _arg(q, dev, n, code), _arg(scale, dev, N * groups, torch.float32), _raw_stream(dev))
 
 
 def rms_norm_grad(N, C, h, rsig, gamma, dy, dh, dgamma, dx):
     """Gradient of rms_norm from its h (x where there was no residual) and rsig; dh, the gradient
     that arrives through h, may be None. dx may be the tensor dy or dh itself."""
     _sizes(N, C)
-    a, tag, n = _Args(), dtype_tag(h), N * C
-    acc, dt = _ACC_DTYPES[tag], h.dtype
+    dev, tag, n, dt = _current_device(), dtype_tag(h), N * C, h.dtype
+    acc = _ACC_DTYPES[tag]
     need = _lib.lib().dragon_hip_rms_norm_grad_scratch_bytes(tag, N, C)
-    ws = a.scratch(need)
-    _call("dragon_hip_rms_norm_grad", tag, N, C, a(h, n, dt), a(rsig, N, acc), a(gamma, C, acc),
-          a(dy, n, dt), a(dh, n, dt, True), a(dgamma, C, acc), a(dx, n, dt),
-          None if ws is None else ws.data_ptr(), need, a.stream())
+    ws = _scratch_for(dev, need)
+    _run("dragon_hip_rms_norm_grad", tag, N, C, _arg(h, dev, n, dt), _arg(rsig, dev, N, acc),
+         _arg(gamma, dev, C, acc), _arg(dy, dev, n, dt), _opt(dh, dev, n, dt), _arg(dgamma, dev, C, acc),
+         _arg(dx, dev, n, dt), None if ws is None else ws.data_ptr(), need, _raw_stream(dev))
 
 
 def _normalizer(reduction, N):
@@ -393,24 +414,26 @@ def topk_distillation_loss_forward(N, C, K, temperature, reduction, x, index, te
     [N, K]; entries outside [0, C) are not listed, rows that list nothing are ignored. stats
     [N + 1] is for the backward call."""
     _sizes(N, C, K)
-    a, tag = _Args(), dtype_tag(x)
+    dev, tag = _current_device(), dtype_tag(x)
     acc, normalizer = _ACC_DTYPES[tag], _normalizer(reduction, N)
     need = _lib.lib().dragon_hip_topk_distillation_loss_scratch_bytes(tag, N, C)
-    ws = a.scratch(need)
-    _call("dragon_hip_topk_distillation_loss_forward", tag, target_tag(index), N, C, K, temperature,
-          normalizer, a(x, N * C, x.dtype), a(index, N * K, index.dtype), a(teacher, N * K, acc),
-          a(stats, N + 1, acc), a(loss, 1 if normalizer else N, acc),
-          None if ws is None else ws.data_ptr(), need, a.stream())
+    ws = _scratch_for(dev, need)
+    _run("dragon_hip_topk_distillation_loss_forward", tag, target_tag(index), N, C, K, temperature,
+         normalizer, _arg(x, dev, N * C, x.dtype), _arg(index, dev, N * K, index.dtype),
+         _arg(teacher, dev, N * K, acc), _arg(stats, dev, N + 1, acc),
+         _arg(loss, dev, 1 if normalizer else N, acc), None if ws is None else ws.data_ptr(), need,
+         _raw_stream(dev))
 
 
 def topk_distillation_loss_backward(N, C, K, temperature, reduction, x, index, teacher, stats, dl, dx):
     """Gradient with respect to x; dx may be the tensor x itself."""
     _sizes(N, C, K)
-    a, tag = _Args(), dtype_tag(x)
+    dev, tag = _current_device(), dtype_tag(x)
     acc, normalizer = _ACC_DTYPES[tag], _normalizer(reduction, N)
-    _call("dragon_hip_topk_distillation_loss_backward", tag, target_tag(index), N, C, K, temperature,
-          normalizer, a(x, N * C, x.dtype), a(index, N * K, index.dtype), a(teacher, N * K, acc),
-          a(stats, N + 1, acc), a(dl, 1 if normalizer else N, acc), a(dx, N * C, x.dtype), a.stream())
+    _run("dragon_hip_topk_distillation_loss_backward", tag, target_tag(index), N, C, K, temperature,
+         normalizer, _arg(x, dev, N * C, x.dtype), _arg(index, dev, N * K, index.dtype),
+         _arg(teacher, dev, N * K, acc), _arg(stats, dev, N + 1, acc),
+         _arg(dl, dev, 1 if normalizer else N, acc), _arg(dx, dev, N * C, x.dtype), _raw_stream(dev))
 
 
 def draft_verify(B, K, C, target, draft, drafted, lengths, u_accept, u_sample, tokens, accepted):
@@ -418,14 +441,13 @@ def draft_verify(B, K, C, target, draft, drafted, lengths, u_accept, u_sample, t
     (None: drafted without sampling): tokens [B, K + 1] = the accepted ones, one that is sampled
     where they end, -1 behind it; accepted [B] = how many. lengths [B] may be None (K each)."""
     _sizes(B, K, C)
-    a, tag = _Args(), dtype_tag(target)
-    dt, it = target.dtype, tokens.dtype
+    dev, tag, dt, it, f32 = _current_device(), dtype_tag(target), target.dtype, tokens.dtype, torch.float32
     need = _lib.lib().dragon_hip_draft_verify_scratch_bytes(tag, B, K, C)
-    ws = a.scratch(need)
-    _call("dragon_hip_draft_verify", tag, target_tag(tokens), B, K, C, a(target, B * (K + 1) * C, dt),
-          a(draft, B * K * C, dt, True), a(drafted, B * K, it), a(lengths, B, it, True),
-          a(u_accept, B * K, torch.float32), a(u_sample, B, torch.float32), a(tokens, B * (K + 1), it),
-          a(accepted, B, it), None if ws is None else ws.data_ptr(), need, a.stream())
+    ws = _scratch_for(dev, need)
+    _run("dragon_hip_draft_verify", tag, target_tag(tokens), B, K, C, _arg(target, dev, B * (K + 1) * C, dt),
+         _opt(draft, dev, B * K * C, dt), _arg(drafted, dev, B * K, it), _opt(lengths, dev, B, it),
+         _arg(u_accept, dev, B * K, f32), _arg(u_sample, dev, B, f32), _arg(tokens, dev, B * (K + 1), it),
+         _arg(accepted, dev, B, it), None if ws is None else ws.data_ptr(), need, _raw_stream(dev))
 
 
 # ---------------------------------------------------------------- fused operator bodies
