@@ -266,16 +266,16 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
   __shared__ A slots[2][2][kThreads / kWaveSize];
   const RowPackets<T, kTPR, kVPT, kRagged> tile(C);
   const A inv_c = A(1) / A(C);
-  A g[kVPT][kVec];
-  if constexpr (kAhead) {
-#pragma unroll
-    for (int s = 0; s < kVPT; ++s) tile.params(gamma, s, g[s]);
-  }
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR;
   u32x4 px[kVPT], pr[kVPT];
   tile.load(x + (row < N ? row : 0) * C, px);
   if constexpr (kResidual) tile.load(residual + (row < N ? row : 0) * C, pr);
+  A g[kVPT][kVec];
+  if constexpr (kAhead) {
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s) tile.params(gamma, s, g[s]);
+  }
   int turn = 0;
   // the trip count is the same for every row of a workgroup: the reductions hold barriers
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < N; base += step) {
@@ -368,6 +368,9 @@ constexpr int64_t kMaxTilePackets = 4096;
 // twenty-four): bf16 [8192, 8192] with a residual 109 us at four, 91 at eight, 92 at twenty-four, 99
 // with a workgroup per row; its gradient at [8192, 4096] 49 us at eight, 53 at sixteen, 58 at
 // thirty-two. More streams at a time are further apart in memory, and leave more partial sums.
+#ifndef RGM
+#define RGM 1
+#endif
 inline int64_t rms_grid(int threads) {
   return static_cast<int64_t>(num_cus()) * (threads < 512 ? 512 / threads : 1);
 }
@@ -379,7 +382,7 @@ int launch_rms_tile(int64_t N, int64_t C, float eps, const void* x, const void* 
   using A = typename IO<T>::Acc;
   constexpr int kThreads = tile_threads(kTPR);
   const int64_t want = ceil_div(N, kThreads / kTPR);
-  const int64_t most = rms_grid(kThreads);
+  const int64_t most = rms_grid(kThreads) * (kRagged ? RGM : 1);
   note_number("threads_per_row", kTPR);
   note_number("packets", kVPT);
   hipLaunchKernelGGL((rms_norm_rows<T, kTPR, kVPT, kRagged, kResidual, kOut>),
@@ -581,6 +584,18 @@ __global__ __launch_bounds__(grad_threads(kTPR)) void rms_norm_grad_rows(
       word_at(s, w) = IO<A>::pack(part);
     }
   };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR;
+  u32x4 ph[kVPT], py[kVPT], pd[kVPT];
+  A rs_next;
+  auto request = [&](int64_t r) {
+    r = r < N ? r : 0;
+    tile.load(h + r * C, ph);
+    tile.load(dy + r * C, py);
+    if constexpr (kThrough) tile.load(dh + r * C, pd);
+    rs_next = rsig[r];
+  };
+  request(row);  // the first row comes while gamma is laid out
   A acc[kVPT][kVec];
 #pragma unroll
   for (int s = 0; s < kVPT; ++s) {
@@ -593,18 +608,6 @@ __global__ __launch_bounds__(grad_threads(kTPR)) void rms_norm_grad_rows(
     for (int e = 0; e < kVec; ++e) acc[s][e] = A(0);
   }
   __syncthreads();
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR;
-  u32x4 ph[kVPT], py[kVPT], pd[kVPT];
-  A rs_next;
-  auto request = [&](int64_t r) {
-    r = r < N ? r : 0;
-    tile.load(h + r * C, ph);
-    tile.load(dy + r * C, py);
-    if constexpr (kThrough) tile.load(dh + r * C, pd);
-    rs_next = rsig[r];
-  };
-  request(row);
   int turn = 0;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < N; base += step) {
     const bool valid = row < N;
@@ -655,10 +658,22 @@ __global__ __launch_bounds__(grad_threads(kTPR)) void rms_norm_grad_rows(
     turn ^= 1;
     if constexpr (!kAhead) request(row);
   }
-  // one group after the other adds its sums; the last of them holds the workgroup's
-  for (int r = 0; kRows > 1 && r < kRows; ++r) {
+  // the rows of a wavefront first: lanes that own the same columns
+#pragma unroll
+  for (int o = kTPR; o < kWaveSize; o <<= 1) {
+#pragma unroll
+    for (int s = 0; s < kVPT; ++s)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) acc[s][e] += __shfl_xor(acc[s][e], o, kWaveSize);
+  }
+  // then one wavefront (or group of them) after the other adds its sums; the last holds the
+  // workgroup's
+  constexpr int kOwners = kTPR < kWaveSize ? kThreads / kWaveSize : kRows;
+  const int owner = kTPR < kWaveSize ? static_cast<int>(threadIdx.x) / kWaveSize : mine;
+  const bool first_rows = static_cast<int>(threadIdx.x) % kWaveSize < kTPR;  // of a wavefront's
+  for (int r = 0; kOwners > 1 && r < kOwners; ++r) {
     __syncthreads();
-    if (mine != r) continue;
+    if (owner != r || !first_rows) continue;
 #pragma unroll
     for (int s = 0; s < kVPT; ++s) {
       if (r > 0) {
@@ -667,10 +682,10 @@ __global__ __launch_bounds__(grad_threads(kTPR)) void rms_norm_grad_rows(
 #pragma unroll
         for (int e = 0; e < kVec; ++e) acc[s][e] += before[e];
       }
-      if (r + 1 < kRows) write_words(s, acc[s]);
+      if (r + 1 < kOwners) write_words(s, acc[s]);
     }
   }
-  if (mine != kRows - 1) return;
+  if (owner != kOwners - 1 || !first_rows) return;
   A* out = partial + static_cast<int64_t>(blockIdx.x) * C;
 #pragma unroll
   for (int s = 0; s < kVPT; ++s) {

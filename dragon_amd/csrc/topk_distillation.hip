@@ -262,10 +262,22 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
       for (int k = 0; k < kUnroll; ++k) IO<T>::unpack(raw[k], v[k]);
       take_packets<T, kUnroll>(v, scale, run);
     }
-    for (p += lane; p < end; p += kTPR) {
-      A v[1][kVec];
-      load_unpack<T>(body + p * kVec, v[0]);
-      take_packets<T, 1>(v, scale, run);
+    if (p < end) {  // what is left, requested at once too
+      u32x4 raw[kUnroll];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        const int64_t at = p + k * kTPR + lane;
+        raw[k] = load_packet(body + (at < end ? at : p) * kVec);
+      }
+      A v[kUnroll][kVec];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        const bool on = p + k * kTPR + lane < end;
+        IO<T>::unpack(raw[k], v[k]);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[k][e] = on ? v[k][e] : acc_neg_inf<A>();
+      }
+      take_packets<T, kUnroll>(v, scale, run);
     }
     run = group_join<T, kTPR>(run, slots);
     if constexpr (kWhole) {
@@ -318,7 +330,8 @@ struct SegmentPlan {
 inline SegmentPlan plan_segments(int64_t N, int64_t C, int64_t K, int vec) {
   const int64_t packets = ceil_div(C, vec);
   if (packets <= 512) return {K <= kWaveK, 1, packets};
-  const int64_t fewest = ceil_div(packets, 2048), most = ceil_div(packets, 1024);
+  // up to 2048 packets a row is one segment: a second launch costs more than the wait for them
+  const int64_t fewest = ceil_div(packets, 2048), most = packets <= 2048 ? 1 : ceil_div(packets, 1024);
   int64_t segments = ceil_div(static_cast<int64_t>(num_cus()) * 8, N > 0 ? N : 1);
   segments = segments < fewest ? fewest : (segments > most ? most : segments);
   const int64_t each = ceil_div(packets, segments);
@@ -512,16 +525,36 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
       asm volatile("" : "+v"(kept[i]));
     }
     group_sync<kTPR>();
+    // the share of a class is that of every entry of it, four entries at a time
+    bool some = false;
+    A share[kSlots];
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      if (!here[i]) continue;
-      A share = A(0);  // of every entry of this class
-      for (int k = 0; k < padded; k += 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) share += classes[k + j] == entries.cls[i] ? shares[k + j] : A(0);
-      }
-      kept[i] = w * (Math::term(kept[i], scale, base) - share);
+      some |= here[i];
+      share[i] = A(0);
     }
+    if (some) {
+#pragma unroll 2
+      for (int k = 0; k < padded; k += 4) {
+        int cls[4];
+        A of[4];
+        const u32x4 packed = *reinterpret_cast<const u32x4_any*>(classes + k);
+        cls[0] = packed.x, cls[1] = packed.y, cls[2] = packed.z, cls[3] = packed.w;
+#pragma unroll
+        for (int j = 0; j < 4; j += 16 / static_cast<int>(sizeof(A))) {
+          A part[16 / sizeof(A)];
+          IO<A>::unpack(*reinterpret_cast<const u32x4_any*>(shares + k + j), part);
+#pragma unroll
+          for (int e = 0; e < static_cast<int>(16 / sizeof(A)); ++e) of[j + e] = part[e];
+        }
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) share[i] += cls[j] == entries.cls[i] ? of[j] : A(0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) kept[i] = w * (Math::term(kept[i], scale, base) - share[i]);
     if (first && lane < cut.head) IO<T>::store1(out + lane, w * Math::term(head, scale, base));
     if (first && lane < cut.tail) IO<T>::store1(out + tail_at, w * Math::term(tail, scale, base));
 #pragma unroll
