@@ -511,6 +511,9 @@ int dragon_hip_draft_verify(int dtype, int index_dtype, int64_t B, int64_t K, in
   if (B == 0) return DRAGON_HIP_OK;
   if (!target || !u_sample || !tokens || !accepted || (K > 0 && (!drafted || !u_accept)))
     return DRAGON_HIP_EINVAL;
+  // several workgroups read the inputs of a sequence whose outputs one of them writes
+  if (accepted == lengths || accepted == drafted || tokens == drafted || tokens == lengths || tokens == accepted)
+    return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_DTYPE(dtype, launch_verify_index, index_dtype, B, K, C, target, draft, drafted,
                             lengths, u_accept, u_sample, tokens, accepted, scratch, scratch_bytes, s);

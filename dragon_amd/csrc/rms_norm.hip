@@ -197,11 +197,17 @@ struct RowPackets {
     }
   }
   __device__ __forceinline__ bool counts(int s, int e) const { return !kRagged || e >= dup[s]; }
-  // Slots without a packet hold the row's first: they are masked where they are used.
+  // Slots without a packet hold the row's first: they are masked where they are used. Packets that
+  // straddle cache lines share them with the neighbouring wavefronts' packets: with the
+  // non-temporal hint of whole lines fp32 [9870, 1001] takes 30 us forward, without 26 (the
+  // gradient, which reads three tensors for one that it writes, 32 and 32.5: kOnce there).
+  template <bool kOnce>
   __device__ __forceinline__ void load(const T* row, u32x4 (&p)[kVPT]) const {
 #pragma unroll
     for (int s = 0; s < kVPT; ++s) {
-      if constexpr (kRagged) {
+      if constexpr (kRagged && !kOnce) {
+        p[s] = load_packet_unaligned(row + col[s]);
+      } else if constexpr (kRagged) {
         p[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_unaligned*>(row + col[s]));
       } else {
         p[s] = load_packet(row + col[s]);
@@ -269,8 +275,8 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR;
   u32x4 px[kVPT], pr[kVPT];
-  tile.load(x + (row < N ? row : 0) * C, px);
-  if constexpr (kResidual) tile.load(residual + (row < N ? row : 0) * C, pr);
+  tile.template load<false>(x + (row < N ? row : 0) * C, px);
+  if constexpr (kResidual) tile.template load<false>(residual + (row < N ? row : 0) * C, pr);
   A g[kVPT][kVec];
   if constexpr (kAhead) {
 #pragma unroll
@@ -298,8 +304,8 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
     }
     const int64_t next = row + step;
     if constexpr (kAhead) {
-      tile.load(x + (next < N ? next : 0) * C, px);
-      if constexpr (kResidual) tile.load(residual + (next < N ? next : 0) * C, pr);
+      tile.template load<false>(x + (next < N ? next : 0) * C, px);
+      if constexpr (kResidual) tile.template load<false>(residual + (next < N ? next : 0) * C, pr);
     }
     sum = row_allreduce<kTPR>(sum, SumOp(), slots[turn][0]);
     const A rs = acc_rsqrt_exact(sum * inv_c + eps);
@@ -340,8 +346,8 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
     row = next;
     turn ^= 1;
     if constexpr (!kAhead) {
-      tile.load(x + (row < N ? row : 0) * C, px);
-      if constexpr (kResidual) tile.load(residual + (row < N ? row : 0) * C, pr);
+      tile.template load<false>(x + (row < N ? row : 0) * C, px);
+      if constexpr (kResidual) tile.template load<false>(residual + (row < N ? row : 0) * C, pr);
     }
   }
 }
@@ -368,9 +374,8 @@ constexpr int64_t kMaxTilePackets = 4096;
 // twenty-four): bf16 [8192, 8192] with a residual 109 us at four, 91 at eight, 92 at twenty-four, 99
 // with a workgroup per row; its gradient at [8192, 4096] 49 us at eight, 53 at sixteen, 58 at
 // thirty-two. More streams at a time are further apart in memory, and leave more partial sums.
-#ifndef RGM
-#define RGM 1
-#endif
+// Quantised rows that are not whole packets, which compute more per byte, take twice as many:
+// fp16 [19870, 805] in groups of 128 columns 25.0 us at eight, 22.7 at sixteen.
 inline int64_t rms_grid(int threads) {
   return static_cast<int64_t>(num_cus()) * (threads < 512 ? 512 / threads : 1);
 }
@@ -382,7 +387,7 @@ int launch_rms_tile(int64_t N, int64_t C, float eps, const void* x, const void* 
   using A = typename IO<T>::Acc;
   constexpr int kThreads = tile_threads(kTPR);
   const int64_t want = ceil_div(N, kThreads / kTPR);
-  const int64_t most = rms_grid(kThreads) * (kRagged ? RGM : 1);
+  const int64_t most = rms_grid(kThreads) * (kRagged && kOut != kPlain ? 2 : 1);
   note_number("threads_per_row", kTPR);
   note_number("packets", kVPT);
   hipLaunchKernelGGL((rms_norm_rows<T, kTPR, kVPT, kRagged, kResidual, kOut>),
@@ -590,9 +595,9 @@ __global__ __launch_bounds__(grad_threads(kTPR)) void rms_norm_grad_rows(
   A rs_next;
   auto request = [&](int64_t r) {
     r = r < N ? r : 0;
-    tile.load(h + r * C, ph);
-    tile.load(dy + r * C, py);
-    if constexpr (kThrough) tile.load(dh + r * C, pd);
+    tile.template load<true>(h + r * C, ph);
+    tile.template load<true>(dy + r * C, py);
+    if constexpr (kThrough) tile.template load<true>(dh + r * C, pd);
     rs_next = rsig[r];
   };
   request(row);  // the first row comes while gamma is laid out
@@ -636,6 +641,11 @@ __global__ __launch_bounds__(grad_threads(kTPR)) void rms_norm_grad_rows(
     }
     const int64_t next = row + step;
     if constexpr (kAhead) request(next);
+    if constexpr (kRagged && kThrough) {
+      // dh has arrived before another wavefront may write dx over elements that both hold
+#pragma unroll
+      for (int s = 0; s < kVPT; ++s) asm volatile("" : "+v"(cd[s]));
+    }
     dot = row_allreduce<kTPR>(dot, SumOp(), slots[turn]);
     const A c = dot * inv_c * rs * rs;
 #pragma unroll

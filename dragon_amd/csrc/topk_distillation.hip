@@ -18,7 +18,6 @@ namespace {
 
 constexpr int kMaxK = 1024;  // entries that a workgroup holds
 
-
 // How exponentials of logits at a temperature are taken. `scale` turns a logit into the domain
 // that running maxima m are held in; term(x) is exp of the logit x relative to m, shrink(d) the
 // factor that a maximum which grows by -d leaves to a sum.
@@ -319,10 +318,9 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_join(
 }
 
 // How a row is cut into segments. A wavefront takes rows of up to 512 packets whole, if it holds
-// the entries. Longer rows are
-// read by workgroups, 2048 packets (8 per thread) at most at a time (of [4096, 131072] bf16: 153 us;
-// 4096 packets 155, 1024 163, for the entries that each reads), and 1024 at least where there
-// are too few rows to give every compute unit eight workgroups.
+// the entries. Longer rows are read by workgroups, 2048 packets (8 per thread) at most at a time
+// (bf16 [4096, 131072]: 153 us; 4096 packets 155, 1024 163, for the entries that each reads), and
+// 1024 at least where there are too few rows to give every compute unit eight workgroups.
 struct SegmentPlan {
   bool wave_rows;
   int64_t segments, packets;  // per row, per segment
@@ -612,9 +610,10 @@ int launch_backward(int64_t N, int64_t C, int64_t K, float temperature, float no
 inline bool index_dtype_ok(int t) { return t == DRAGON_HIP_I32 || t == DRAGON_HIP_I64; }
 inline bool dtype_ok(int d) { return d >= DRAGON_HIP_F16 && d <= DRAGON_HIP_F64; }
 inline bool sizes_ok(int64_t N, int64_t C, int64_t K, float temperature, float normalizer) {
-  // a temperature or a normalizer that is NaN fails every comparison
-  return N >= 0 && N < INT_MAX && C > 0 && C <= INT_MAX && K > 0 && K <= kMaxK && temperature > 0.f &&
-      temperature <= 3.4e38f && normalizer == normalizer;
+  // a temperature or a normalizer that is NaN fails every comparison; beyond these bounds the
+  // temperature's reciprocal or square is no 32-bit number
+  return N >= 0 && N < INT_MAX && C > 0 && C <= INT_MAX && K > 0 && K <= kMaxK && temperature > 1e-18f &&
+      temperature < 1e18f && normalizer == normalizer;
 }
 
 // Calls FN<T, IndexT>(args...).

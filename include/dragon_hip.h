@@ -362,8 +362,8 @@ int dragon_hip_rms_norm(int dtype, int64_t N, int64_t C, float eps, const void* 
  * group; the last group of a row may be shorter):
  *   scale = max(max|y|, 1e-30) / 448,  q = e4m3(y / scale)
  * q: one byte per element [N, C]; scale: float[N, ceil(C / group)]. A NaN in y
- * becomes a NaN code and is passed over by the maximum. dtype F16, BF16 or
- * F32 (DRAGON_HIP_EDTYPE otherwise). */
+ * becomes a NaN code and is passed over by the maximum; an infinity makes its
+ * group's scale infinite. dtype F16, BF16 or F32 (DRAGON_HIP_EDTYPE otherwise). */
 int dragon_hip_rms_norm_quant(int dtype, int64_t N, int64_t C, int64_t group, float eps,
                               const void* x, const void* residual, const void* gamma, void* h,
                               void* rsig, void* q, void* scale, void* stream);
@@ -397,8 +397,8 @@ int dragon_hip_rms_norm_grad(int dtype, int64_t N, int64_t C, const void* h, con
  * or the number of rows that are not ignored where normalizer < 0.
  * stats: AccT[N + 1], written by the forward for the backward call: log sum
  * exp(x / t) of each row (+inf for an ignored one), then the divisor (1 for
- * normalizer 0). dx may be the very buffer of x. 1 <= K <= 1024, t > 0, N and C
- * below 2^31. The sums have a fixed order. */
+ * normalizer 0). dx may be the very buffer of x. 1 <= K <= 1024, 1e-18 < t < 1e18,
+ * N and C below 2^31. The sums have a fixed order. */
 size_t dragon_hip_topk_distillation_loss_scratch_bytes(int dtype, int64_t N, int64_t C);
 int dragon_hip_topk_distillation_loss_forward(int dtype, int index_dtype, int64_t N, int64_t C,
                                               int64_t K, float temperature, float normalizer,
@@ -427,7 +427,7 @@ int dragon_hip_topk_distillation_loss_backward(int dtype, int index_dtype, int64
  * tokens (index type, [B, K + 1]) = the n accepted, the sampled one, -1 behind it;
  * accepted (index type, [B]) = n. Probabilities that are negative or not finite count as 0; a
  * drafted token outside [0, C) is refused. Comparisons and sums are held in 64 bits. K may be
- * 0 (draft, drafted, u_accept unused). B, K and C below 2^31. */
+ * 0 (draft, drafted, u_accept unused). B, K and C below 2^31. No output may lie on an input. */
 size_t dragon_hip_draft_verify_scratch_bytes(int dtype, int64_t B, int64_t K, int64_t C);
 int dragon_hip_draft_verify(int dtype, int index_dtype, int64_t B, int64_t K, int64_t C,
                             const void* target, const void* draft, const void* drafted,

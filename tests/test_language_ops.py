@@ -61,7 +61,7 @@ def test_distillation_refusals():
     for f in (fwd, bwd):
         assert f(dtype=4) == EDTYPE and f(it=2) == EDTYPE
         for bad in (dict(N=-1), dict(C=0), dict(k=0), dict(k=1025), dict(t=0.0), dict(t=-2.0), dict(t=float("nan")),
-                    dict(t=float("inf")), dict(norm=float("nan")), dict(x=None), dict(st=None), dict(C=1 << 31),
+                    dict(t=float("inf")), dict(t=1e-20), dict(t=1e20), dict(norm=float("nan")), dict(x=None), dict(st=None), dict(C=1 << 31),
                     dict(N=(1 << 31) - 1)):
             assert f(**bad) == EINVAL, bad
     assert fwd(loss=None) == EINVAL and bwd(dl=None) == EINVAL and bwd(dx=None) == EINVAL
@@ -78,6 +78,8 @@ def test_draft_verify_refusals():
     for bad in (dict(B=-1), dict(k=-1), dict(C=0), dict(C=1 << 31), dict(t=None), dict(d=None), dict(ua=None),
                 dict(us=None), dict(tok=None), dict(acc=None)):
         assert call(**bad) == EINVAL, bad
+    for bad in (dict(acc=P[3]), dict(acc=P[2]), dict(tok=P[2]), dict(tok=P[3]), dict(tok=P[7])):  # outputs on inputs
+        assert call(**bad) == EINVAL, bad
     assert call(B=0) == 0
 
 
@@ -88,6 +90,29 @@ def test_every_operator_has_a_plan():
         assert "[" in K.plan_name(op, "bfloat16", dims)
         with pytest.raises(ValueError):
             K.plan_name(op, "bfloat16", (4, -1, 0))
+
+
+def test_plans_by_size():
+    """Which kernels sizes take: rows in registers up to 4096 packets, wavefront rows, segments and parts."""
+    plan = lambda op, dims, dtype="bfloat16": K.plan_name(op, dtype, dims)
+    assert plan("rms_norm", (8, 4096)).startswith("threads_per_row=256:packets=2:rms_norm_rows<")
+    assert plan("rms_norm", (8, 64)).startswith("threads_per_row=8:packets=1:")
+    assert plan("rms_norm", (8, 32768)).startswith("threads_per_row=1024:packets=4:")
+    assert "rms_norm_rows_looped" in plan("rms_norm", (8, 32769)) and "looped" in plan("rms_norm", (8, 7))
+    assert "rms_norm_rows_looped" in plan("rms_norm_quant", (8, 40000, 128))
+    assert "grad_rows" in plan("rms_norm_grad", (8, 16384)) and "grad_dots" in plan("rms_norm_grad", (8, 16392))
+    assert "grad_rows" in plan("rms_norm_grad", (8, 16384), "float32")
+    f, b = "topk_distillation_loss_forward", "topk_distillation_loss_backward"
+    assert "IndexT,64,1,true" in plan(f, (100, 4096, 64)) and "IndexT,64,4,true" in plan(f, (100, 4096, 256))
+    assert "IndexT,256,4,true" in plan(f, (100, 4096, 257)) and "IndexT,256,1,true" in plan(f, (100, 16384, 64))
+    assert "IndexT,256,1,false" in plan(f, (100, 16392, 64)) and "distill_forward_join<T,IndexT,64,1>" in plan(f, (100, 16392, 64))
+    assert "distill_forward_join<T,IndexT,256,4>" in plan(f, (100, 131072, 1024))
+    assert "IndexT,64,4,1" in plan(b, (100, 2048, 64)) and "IndexT,64,8,4" in plan(b, (100, 4096, 65))
+    assert "IndexT,256,2,1" in plan(b, (100, 131072, 64)) and "IndexT,256,4,4" in plan(b, (100, 131072, 300))
+    assert "draft_verify_rows" in plan("draft_verify", (1, 4, 32768), "float32")
+    assert "draft_verify_runs" in plan("draft_verify", (1, 4, 32769), "float32")
+    assert "draft_verify_rows" in plan("draft_verify", (512, 4, 131072), "float32")
+    assert "draft_verify_runs" in plan("draft_verify", (512, 4, 1 << 20), "float32")
 
 
 # ---------------------------------------------------------------- the plain forms themselves
