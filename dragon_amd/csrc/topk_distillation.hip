@@ -40,11 +40,18 @@ struct ExpMath {
     else return acc_exp(d);
   }
   static __device__ __forceinline__ A term(A x, A scale, A m) { return shrink(fma(x, scale, -m)); }
-  // log of a sum relative to m, and a natural logarithm in the domain of m
+  // log of a sum s relative to m; its two parts, and how far a logit lies below m, apart: the loss
+  // adds these, which are smaller than the logarithm itself and lose less in rounding
   static __device__ __forceinline__ A log_of(A m, A s) {
-    if constexpr (kBase2) return (m + __builtin_amdgcn_logf(s)) * kLn2;
+    if constexpr (kBase2) return fma(m, kLn2, acc_log(s));
     return m + acc_log(s);
   }
+  static __device__ __forceinline__ A below(A x, A scale, A m) {
+    const A d = fma(-x, scale, m);
+    if constexpr (kBase2) return d * kLn2;
+    return d;
+  }
+  // a natural logarithm in the domain of m
   static __device__ __forceinline__ A from_log(A l) {
     if constexpr (kBase2) return l * kLog2e;
     return l;
@@ -190,18 +197,19 @@ __device__ __forceinline__ void finish_row(const int64_t row, const int64_t C,
   A xk[kSlots];
 #pragma unroll
   for (int i = 0; i < kSlots; ++i)
-    xk[i] = entries.cls[i] >= 0 ? IO<T>::load1(x + row * C + entries.cls[i]) * inv_t : A(0);
+    xk[i] = entries.cls[i] >= 0 ? IO<T>::load1(x + row * C + entries.cls[i]) : A(0);
   const ExpSum<A> t = entries.sum(slots);
   const A log_total = acc_log(t.s);
   // a row of nothing but -inf has no distribution
   const A lse = run.m == acc_neg_inf<A>() ? A(__builtin_nanf("")) : ExpMath<T>::log_of(run.m, run.s);
+  const A scale = ExpMath<T>::scale(inv_t), log_s = acc_log(run.s);
   A part = A(0);
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
     if (entries.cls[i] < 0) continue;
     const A log_p = entries.z[i] - t.m - log_total;
     const A p = acc_exp(log_p);
-    if (p != A(0)) part += p * (log_p - xk[i] + lse);
+    if (p != A(0)) part += p * (log_p + (ExpMath<T>::below(xk[i], scale, run.m) + log_s));
   }
   part = group_reduce<kTPR>(part, SumOp(), slots[2]);
   if (threadIdx.x % kTPR == 0) {
