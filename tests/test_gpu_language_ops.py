@@ -720,6 +720,64 @@ def test_two_streams_at_once():
             assert torch.equal(t[n].view(torch.uint8), w[n].view(torch.uint8)), n
 
 
+# ---------------------------------------------------------------- sizes at which the launchers change kernels
+
+@pytest.mark.parametrize("dtype,vec", [("bfloat16", 8), ("float32", 4), ("float64", 2)])
+def test_rms_norm_at_the_seams(dtype, vec):
+    """Rows of one packet more or less, and one element more or less, than the tiles hold; groups of rows that
+    are partly filled."""
+    K = _K()
+    for packets in (1, 2, 8, 16, 32, 64, 128, 256, 512, 1024, 2048, 4096):
+        for extra in (-1, 0, 1, vec):
+            C = packets * vec + extra
+            for N in (1, 67 if packets < 64 else 5):
+                x, r, dy = (_make((N, C), dtype, packets + i) for i in range(3))
+                gamma = (1 + _make((C,), "float64", 9, 0.3)).to(L.acc_dtype(dtype))
+                h, y, rsig = torch.empty_like(x), torch.empty_like(x), torch.empty(N, dtype=gamma.dtype, device="cuda")
+                K.rms_norm(N, C, 1e-5, x, r, gamma, h, rsig, y)
+                s, rs, want = L.rms_norm(L.f64(x), L.f64(r), L.f64(gamma), float(np.float32(1e-5)))
+                bh, brs, by = L.rms_norm_bounds(dtype, s, rs, want)
+                L.assert_close(L.f64(h), s, bh, "h %d" % C)
+                L.assert_close(L.f64(rsig), rs, brs, "rsig %d" % C)
+                L.assert_close(L.f64(y), want, by, "y %d" % C)
+                dgamma, dx = torch.empty_like(gamma), torch.empty_like(x)
+                K.rms_norm_grad(N, C, h, rsig, gamma, dy, r, dgamma, dx)
+                _check_grad(dtype, h, rsig, gamma, dy, r, dgamma, dx)
+                if dtype != "float64":
+                    for group in (0, 64):
+                        q = torch.empty((N, C), dtype=torch.float8_e4m3fn, device="cuda")
+                        scale = torch.empty((N, -(-C // group) if group else 1), device="cuda")
+                        K.rms_norm_quant(N, C, group, 1e-5, x, r, gamma, h, rsig, q, scale)
+                        _check_quant(dtype, group, x, r, gamma, h, rsig, q, scale)
+
+
+@pytest.mark.parametrize("dtype,vec", [("bfloat16", 8), ("float32", 4)])
+def test_distillation_at_the_seams(dtype, vec):
+    for packets in (256, 512, 1024, 2048, 2600):
+        for extra in (-1, 0, 1):
+            C = packets * vec + extra
+            for k in (64, 65, 256, 257):
+                x, index, teacher = _distill_case(5, C, k, dtype, torch.int32, C + k)
+                dl = torch.ones(1, device="cuda")
+                _check_distill(dtype, x, index, teacher, 2.0, "VALID", dl, *_run_distill(x, index, teacher, 2.0, "VALID", dl))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32", "float64"])
+def test_draft_verify_at_the_seams(dtype):
+    """Rows that end inside a packet, inside a run of 64 packets and behind one, on both sides of the size from which
+    rows are cut; drafts of 64 positions and more."""
+    for B, k, C in ((3, 2, 7), (3, 2, 8), (3, 2, 511), (3, 2, 513), (2, 2, 32767), (2, 2, 32768), (2, 2, 32769), (2, 1, 65537),
+                    (2, 64, 300), (2, 65, 300), (2, 1, 262145)):
+        for sampled in (True, False):
+            t = _verify_case(B, k, C, dtype, torch.int32, sampled, C + k)
+            if C % 2:
+                t["u_accept"].fill_(0.999)  # refused early
+            _check_verify(t)
+            t["u_sample"].fill_(1 - 2.0 ** -24)
+            t["lengths"].fill_(k)
+            _check_verify(t)
+
+
 def test_arguments_are_checked():
     K = _K()
     from dragon_amd import _lib
