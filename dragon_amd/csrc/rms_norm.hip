@@ -700,9 +700,19 @@ __global__ __launch_bounds__(grad_threads(kTPR)) void rms_norm_grad_rows(
 #pragma unroll
   for (int s = 0; s < kVPT; ++s) {
     if (!tile.on[s]) continue;
+    if (!kRagged || tile.dup[s] == 0) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      if (tile.counts(s, e)) out[tile.col[s] + e] = acc[s][e];
+      for (int w = 0; w < kWords; ++w) {
+        A part[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) part[e] = acc[s][w * kPer + e];
+        *reinterpret_cast<u32x4_unaligned*>(out + tile.col[s] + w * kPer) = IO<A>::pack(part);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        if (e >= tile.dup[s]) out[tile.col[s] + e] = acc[s][e];
+      }
     }
   }
 }

@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
   using A = typename IO<T>::Acc;
   constexpr int kVec = IO<T>::kVec;
   if (!reduced && blockIdx.x == 0 && threadIdx.x == 0) stats[N] = A(1);  // the divisor of single losses
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = 4, kTake = 2;  // packets requested at once, and joined at once
   __shared__ A slots[5][kTPR / kWaveSize];
   constexpr int kRows = kSegmentThreads / kTPR;
   const int lane = static_cast<int>(threadIdx.x) % kTPR;
@@ -264,10 +264,13 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
       u32x4 raw[kUnroll];
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) raw[k] = load_packet(body + (p + k * kTPR + lane) * kVec);
-      A v[kUnroll][kVec];
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) IO<T>::unpack(raw[k], v[k]);
-      take_packets<T, kUnroll>(v, scale, run);
+      for (int k = 0; k < kUnroll; k += kTake) {
+        A v[kTake][kVec];
+#pragma unroll
+        for (int i = 0; i < kTake; ++i) IO<T>::unpack(raw[k + i], v[i]);
+        take_packets<T, kTake>(v, scale, run);
+      }
     }
     if (p < end) {  // what is left, requested at once too
       u32x4 raw[kUnroll];
@@ -276,15 +279,18 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
         const int64_t at = p + k * kTPR + lane;
         raw[k] = load_packet(body + (at < end ? at : p) * kVec);
       }
-      A v[kUnroll][kVec];
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
-        const bool on = p + k * kTPR + lane < end;
-        IO<T>::unpack(raw[k], v[k]);
+      for (int k = 0; k < kUnroll; k += kTake) {
+        A v[kTake][kVec];
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) v[k][e] = on ? v[k][e] : acc_neg_inf<A>();
+        for (int i = 0; i < kTake; ++i) {
+          const bool on = p + (k + i) * kTPR + lane < end;
+          IO<T>::unpack(raw[k + i], v[i]);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) v[i][e] = on ? v[i][e] : acc_neg_inf<A>();
+        }
+        take_packets<T, kTake>(v, scale, run);
       }
-      take_packets<T, kUnroll>(v, scale, run);
     }
     run = group_join<T, kTPR>(run, slots);
     if constexpr (kWhole) {
@@ -325,19 +331,23 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_join(
   }
 }
 
-// How a row is cut into segments. A wavefront takes rows of up to 512 packets whole, if it holds
-// the entries. Longer rows are read by workgroups, 2048 packets (8 per thread) at most at a time
-// (bf16 [4096, 131072]: 153 us; 4096 packets 155, 1024 163, for the entries that each reads), and
-// 1024 at least where there are too few rows to give every compute unit eight workgroups.
+// How a row is cut into segments. A wavefront that holds the entries takes rows of up to 512 packets
+// whole, and of up to 2048 where there are 2048 rows and more (fp16 [5330, 5440]: 27 us by
+// workgroups, 19 by wavefronts). Workgroups take longer rows whole where enough of them fill the
+// device, which saves the second launch (bf16 [4096, 32000] 50 -> 47 us, [1000, 32000] 22 -> 17).
+// Other rows are cut: 2048 packets (8 per thread) at most at a time (bf16 [4096, 131072]: 153 us;
+// 4096 packets 155, 1024 163, for the entries that each reads), and 1024 at least where there
+// are too few rows to give every compute unit eight workgroups.
 struct SegmentPlan {
   bool wave_rows;
   int64_t segments, packets;  // per row, per segment
 };
 inline SegmentPlan plan_segments(int64_t N, int64_t C, int64_t K, int vec) {
   const int64_t packets = ceil_div(C, vec);
-  if (packets <= 512) return {K <= kWaveK, 1, packets};
-  // up to 2048 packets a row is one segment: a second launch costs more than the wait for them
-  const int64_t fewest = ceil_div(packets, 2048), most = packets <= 2048 ? 1 : ceil_div(packets, 1024);
+  const bool waves = K <= kWaveK && packets <= (N >= 2048 ? 2048 : 512);
+  const int64_t whole = N >= 2048 ? 8192 : (N >= 512 ? 4096 : 2048);
+  if (waves || packets <= whole) return {waves, 1, packets};
+  const int64_t fewest = ceil_div(packets, 2048), most = ceil_div(packets, 1024);
   int64_t segments = ceil_div(static_cast<int64_t>(num_cus()) * 8, N > 0 ? N : 1);
   segments = segments < fewest ? fewest : (segments > most ? most : segments);
   const int64_t each = ceil_div(packets, segments);

@@ -103,6 +103,9 @@ def test_plans_by_size():
     assert "grad_rows" in plan("rms_norm_grad", (8, 16384)) and "grad_dots" in plan("rms_norm_grad", (8, 16392))
     assert "grad_rows" in plan("rms_norm_grad", (8, 16384), "float32")
     f, b = "topk_distillation_loss_forward", "topk_distillation_loss_backward"
+    assert "IndexT,64,1,true" in plan(f, (2048, 16384, 64)) and "IndexT,256,1,true" in plan(f, (2047, 16384, 64))
+    assert "IndexT,256,1,true" in plan(f, (2048, 65536, 64)) and "IndexT,256,1,false" in plan(f, (2048, 65544, 64))
+    assert "IndexT,256,1,true" in plan(f, (512, 32768, 64)) and "IndexT,256,1,false" in plan(f, (511, 32768, 64))
     assert "IndexT,64,1,true" in plan(f, (100, 4096, 64)) and "IndexT,64,4,true" in plan(f, (100, 4096, 256))
     assert "IndexT,256,4,true" in plan(f, (100, 4096, 257)) and "IndexT,256,1,true" in plan(f, (100, 16384, 64))
     assert "IndexT,256,1,false" in plan(f, (100, 16392, 64)) and "distill_forward_join<T,IndexT,64,1>" in plan(f, (100, 16392, 64))
