@@ -8,6 +8,7 @@
 // writes the gradient once: both are bound by HBM; the teacher's K entries per row are a few
 // hundred bytes against the row's tens or hundreds of KB.
 #include <climits>
+#include <limits>
 
 #include "row_loop.h"
 #include "row_tile.h"
@@ -41,15 +42,15 @@ struct ExpMath {
   }
   static __device__ __forceinline__ A term(A x, A scale, A m) { return shrink(fma(x, scale, -m)); }
   // log of a sum s relative to m; its two parts, and how far a logit lies below m, apart: the loss
-  // adds these, which are smaller than the logarithm itself and lose less in rounding
+  // adds these, which are smaller than the logarithm itself and lose less in rounding. Halves, so
+  // that the type's lowest value has a distance in the base-2 domain too.
   static __device__ __forceinline__ A log_of(A m, A s) {
     if constexpr (kBase2) return fma(m, kLn2, acc_log(s));
     return m + acc_log(s);
   }
   static __device__ __forceinline__ A below(A x, A scale, A m) {
-    const A d = fma(-x, scale, m);
-    if constexpr (kBase2) return d * kLn2;
-    return d;
+    if constexpr (kBase2) return fma(-x, scale * 0.5f, m * 0.5f) * (2.f * kLn2);
+    return fma(-x, scale, m);
   }
   // a natural logarithm in the domain of m
   static __device__ __forceinline__ A from_log(A l) {
@@ -58,16 +59,21 @@ struct ExpMath {
   }
 };
 
-// A running maximum and the sum of exponentials relative to it. An empty pair, and one of
-// nothing but -inf, is (-inf, 0); a NaN or +inf among the values makes the sum NaN.
+// A running maximum, never below -kFar, and the sum of exponentials relative to it. An empty pair is
+// (-kFar, 0); a NaN or +inf among the values makes the sum NaN.
+//
+// term() multiplies without rounding and subtracts a maximum that was rounded: the term of the
+// maximum itself is exp of that rounding, a part in 10^4 at 2048 and anything from 0 to infinity at
+// the lowest value of a type, which masks are made of. The floor keeps masked stretches of a row
+// (threads, segments) at sums of 0. Rows whose maximum is not inside (-kFar, kFar) are masked all
+// over, or are logits of unusual size: they are read again by far_sum, which subtracts first.
+constexpr int kFar = 2048;
 template <typename A>
 struct ExpSum {
   A m, s;
+  static __device__ __forceinline__ ExpSum none() { return {A(-kFar), A(0)}; }
+  __device__ __forceinline__ bool far() const { return !(m > A(-kFar) && m < A(kFar)); }
 };
-template <typename A>
-__device__ __forceinline__ A finite_base(A m) {
-  return m == acc_neg_inf<A>() ? A(0) : m;
-}
 
 // The kVec logits of kPackets packets joined to a thread's pair: one maximum and one rescaling
 // for all of them.
@@ -82,12 +88,11 @@ __device__ __forceinline__ void take_packets(const typename IO<T>::Acc (&v)[kPac
 #pragma unroll
     for (int e = 0; e < IO<T>::kVec; ++e) top = MaxOp()(top, v[k][e]);
   const A m = MaxOp()(run.m, top * scale);
-  const A base = finite_base(m);
-  A s = run.s * ExpMath<T>::shrink(run.m - base);
+  A s = run.s * ExpMath<T>::shrink(run.m - m);
 #pragma unroll
   for (int k = 0; k < kPackets; ++k)
 #pragma unroll
-    for (int e = 0; e < IO<T>::kVec; ++e) s += ExpMath<T>::term(v[k][e], scale, base);
+    for (int e = 0; e < IO<T>::kVec; ++e) s += ExpMath<T>::term(v[k][e], scale, m);
   run = {m, s};
 }
 template <typename T>
@@ -95,8 +100,7 @@ __device__ __forceinline__ void take_one(const typename IO<T>::Acc v, const type
                                          ExpSum<typename IO<T>::Acc>& run) {
   using A = typename IO<T>::Acc;
   const A m = MaxOp()(run.m, v * scale);
-  const A base = finite_base(m);
-  run = {m, run.s * ExpMath<T>::shrink(run.m - base) + ExpMath<T>::term(v, scale, base)};
+  run = {m, run.s * ExpMath<T>::shrink(run.m - m) + ExpMath<T>::term(v, scale, m)};
 }
 
 // All-reduce over the kTPR threads of a row's group: a wavefront, or a workgroup of several (one
@@ -111,7 +115,7 @@ __device__ __forceinline__ ExpSum<typename IO<T>::Acc> group_join(
     const ExpSum<typename IO<T>::Acc> v, typename IO<T>::Acc (*slots)[kTPR / kWaveSize]) {
   using A = typename IO<T>::Acc;
   const A m = group_reduce<kTPR>(v.m, MaxOp(), slots[0]);
-  return {m, group_reduce<kTPR>(v.s * ExpMath<T>::shrink(v.m - finite_base(m)), SumOp(), slots[1])};
+  return {m, group_reduce<kTPR>(v.s * ExpMath<T>::shrink(v.m - m), SumOp(), slots[1])};
 }
 template <int kTPR>
 __device__ __forceinline__ bool group_any(bool v) {
@@ -133,6 +137,35 @@ struct RowCut {
     tail = static_cast<int>(C - head - packets * IO<T>::kVec);
   }
 };
+
+// A row by itself: its largest logit (not scaled), and the sum of exp((x - that) / t). By the kTPR
+// threads of a group, which read it twice. A row of nothing but -inf, as one with NaN or +inf,
+// has a NaN sum.
+template <typename T, int kTPR>
+__device__ __forceinline__ ExpSum<typename IO<T>::Acc> far_sum(
+    const T* row, int64_t C, typename IO<T>::Acc inv_t, typename IO<T>::Acc (*slots)[kTPR / kWaveSize]) {
+  using A = typename IO<T>::Acc;
+  constexpr int kVec = IO<T>::kVec;
+  const int lane = static_cast<int>(threadIdx.x) % kTPR;
+  A m = acc_neg_inf<A>(), s = A(0);
+#pragma unroll 1
+  for (int64_t col = static_cast<int64_t>(lane) * kVec; col < C; col += kTPR * kVec) {
+    A v[kVec];
+    load_span<T>(row + col, span_of(C - col, kVec), acc_neg_inf<A>(), v);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) m = MaxOp()(m, v[e]);
+  }
+  m = group_reduce<kTPR>(m, MaxOp(), slots[0]);
+#pragma unroll 1
+  for (int64_t col = static_cast<int64_t>(lane) * kVec; col < C; col += kTPR * kVec) {
+    const int n = span_of(C - col, kVec);
+    A v[kVec];
+    load_span<T>(row + col, n, A(0), v);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) s += e < n ? acc_exp((v[e] - m) * inv_t) : A(0);
+  }
+  return {m, group_reduce<kTPR>(s, SumOp(), slots[1])};
+}
 
 // The teacher's entries of a row in the registers of its group, one or four to a thread (four
 // where K asks for them: they cost a kernel's occupancy): entry k belongs to thread k % kTPR, in
@@ -200,16 +233,27 @@ __device__ __forceinline__ void finish_row(const int64_t row, const int64_t C,
     xk[i] = entries.cls[i] >= 0 ? IO<T>::load1(x + row * C + entries.cls[i]) : A(0);
   const ExpSum<A> t = entries.sum(slots);
   const A log_total = acc_log(t.s);
-  // a row of nothing but -inf has no distribution
-  const A lse = run.m == acc_neg_inf<A>() ? A(__builtin_nanf("")) : ExpMath<T>::log_of(run.m, run.s);
-  const A scale = ExpMath<T>::scale(inv_t), log_s = acc_log(run.s);
+  const A scale = ExpMath<T>::scale(inv_t);
+  A log_s = acc_log(run.s), lse = ExpMath<T>::log_of(run.m, run.s);
+  const bool far = run.far();
+  A largest = A(0);
+  if (far) {
+    const ExpSum<A> own = far_sum<T, kTPR>(x + row * C, C, inv_t, slots + 3);
+    largest = own.m;
+    log_s = acc_log(own.s);
+    lse = largest * inv_t + log_s;
+    // finite, though x / t may not be: +inf stands for an ignored row
+    const A most = std::numeric_limits<A>::max();
+    lse = lse > most ? most : (lse < -most ? -most : lse);
+  }
   A part = A(0);
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
     if (entries.cls[i] < 0) continue;
     const A log_p = entries.z[i] - t.m - log_total;
     const A p = acc_exp(log_p);
-    if (p != A(0)) part += p * (log_p + (ExpMath<T>::below(xk[i], scale, run.m) + log_s));
+    const A below = far ? (largest - xk[i]) * inv_t : ExpMath<T>::below(xk[i], scale, run.m);
+    if (p != A(0)) part += p * (log_p + (below + log_s));
   }
   part = group_reduce<kTPR>(part, SumOp(), slots[2]);
   if (threadIdx.x % kTPR == 0) {
@@ -233,7 +277,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
   constexpr int kVec = IO<T>::kVec;
   if (!reduced && blockIdx.x == 0 && threadIdx.x == 0) stats[N] = A(1);  // the divisor of single losses
   constexpr int kUnroll = 4, kTake = 2;  // packets requested at once, and joined at once
-  __shared__ A slots[5][kTPR / kWaveSize];
+  __shared__ A slots[7][kTPR / kWaveSize];
   constexpr int kRows = kSegmentThreads / kTPR;
   const int lane = static_cast<int>(threadIdx.x) % kTPR;
   const A scale = ExpMath<T>::scale(inv_t);
@@ -253,7 +297,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_segments(
     const T* xr = x + row * C;
     const RowCut<T> cut(xr, C);
     const T* body = xr + cut.head;
-    ExpSum<A> run = {acc_neg_inf<A>(), A(0)};
+    ExpSum<A> run = ExpSum<A>::none();
     int64_t p = segment * segment_packets;
     const int64_t end = p + segment_packets < cut.packets ? p + segment_packets : cut.packets;
     if (segment == 0) {
@@ -311,19 +355,18 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_forward_join(
     typename IO<T>::Acc* __restrict__ loss, const ExpSum<typename IO<T>::Acc>* __restrict__ pairs) {
   using A = typename IO<T>::Acc;
   constexpr int kRows = kSegmentThreads / kTPR;
-  __shared__ A slots[5][kTPR / kWaveSize];
+  __shared__ A slots[7][kTPR / kWaveSize];
   const int lane = static_cast<int>(threadIdx.x) % kTPR;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; row < N;
        row += static_cast<int64_t>(gridDim.x) * kRows) {
     Entries<T, IndexT, kTPR, kSlots> entries;
     entries.load(row, C, K, inv_t, index, teacher);
     if (!entries.any()) continue;  // written by the row's first segment, which left no pair
-    ExpSum<A> run = {acc_neg_inf<A>(), A(0)};
+    ExpSum<A> run = ExpSum<A>::none();
     for (int i = lane; i < segments; i += kTPR) {
       const ExpSum<A> other = pairs[row * segments + i];
       const A m = MaxOp()(run.m, other.m);
-      const A base = finite_base(m);
-      run = {m, run.s * ExpMath<T>::shrink(run.m - base) + other.s * ExpMath<T>::shrink(other.m - base)};
+      run = {m, run.s * ExpMath<T>::shrink(run.m - m) + other.s * ExpMath<T>::shrink(other.m - m)};
     }
     run = group_join<T, kTPR>(run, slots);
     finish_row<T, IndexT, kTPR, kSlots>(row, C, inv_t, t2, x, entries, run, stats, loss, slots + 2);
@@ -454,6 +497,99 @@ __device__ __forceinline__ void group_sync() {
   }
 }
 
+// The teacher's shares by the threads of a row's group, through its LDS (classes and shares of the K
+// entries, padded to a multiple of 4): share[i] is that of the class of the thread's entry i, which
+// is the share of every entry of it, four entries at a time, where wanted[i]. It comes back behind a
+// barrier of the group.
+template <typename T, typename IndexT, int kTPR, int kSlots>
+__device__ __forceinline__ void sum_shares(const Entries<T, IndexT, kTPR, kSlots>& entries, const int padded,
+                                           const bool (&wanted)[kSlots], int* classes,
+                                           typename IO<T>::Acc* shares,
+                                           typename IO<T>::Acc (*slots)[kTPR / kWaveSize],
+                                           typename IO<T>::Acc (&kept)[kSlots],
+                                           typename IO<T>::Acc (&share)[kSlots]) {
+  using A = typename IO<T>::Acc;
+  const int lane = static_cast<int>(threadIdx.x) % kTPR;
+  const ExpSum<A> t = entries.sum(slots);
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    const int k = i * kTPR + lane;
+    if (k < padded) {
+      classes[k] = entries.cls[i];
+      shares[k] = entries.cls[i] >= 0 ? acc_exp(entries.z[i] - t.m) / t.s : A(0);
+    }
+    // its logit has arrived before another thread may write over it
+    asm volatile("" : "+v"(kept[i]));
+  }
+  group_sync<kTPR>();
+  bool some = false;
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    some |= wanted[i];
+    share[i] = A(0);
+  }
+  if (some) {
+#pragma unroll 2
+    for (int k = 0; k < padded; k += 4) {
+      int cls[4];
+      A of[4];
+      const u32x4 packed = *reinterpret_cast<const u32x4_any*>(classes + k);
+      cls[0] = packed.x, cls[1] = packed.y, cls[2] = packed.z, cls[3] = packed.w;
+#pragma unroll
+      for (int j = 0; j < 4; j += 16 / static_cast<int>(sizeof(A))) {
+        A part[16 / sizeof(A)];
+        IO<A>::unpack(*reinterpret_cast<const u32x4_any*>(shares + k + j), part);
+#pragma unroll
+        for (int e = 0; e < static_cast<int>(16 / sizeof(A)); ++e) of[j + e] = part[e];
+      }
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) share[i] += cls[j] == entries.cls[i] ? of[j] : A(0);
+    }
+  }
+}
+
+// The gradient of a row whose log-sum is so large that its rounding would show in the exponentials: its
+// largest logit and sum are found anew, and one group takes the whole row, which no other reads or
+// writes, so that dx may lie on x.
+template <typename T, typename IndexT, int kTPR, int kSlots>
+__device__ __forceinline__ void far_row(const T* in, T* out, const int64_t C, const int padded,
+                                        const Entries<T, IndexT, kTPR, kSlots>& entries,
+                                        const typename IO<T>::Acc inv_t, const typename IO<T>::Acc w,
+                                        int* classes, typename IO<T>::Acc* shares,
+                                        typename IO<T>::Acc (*slots)[kTPR / kWaveSize]) {
+  using A = typename IO<T>::Acc;
+  constexpr int kVec = IO<T>::kVec;
+  const int lane = static_cast<int>(threadIdx.x) % kTPR;
+  A kept[kSlots], share[kSlots];
+  bool here[kSlots];
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    here[i] = entries.cls[i] >= 0;
+    kept[i] = here[i] ? IO<T>::load1(in + entries.cls[i]) : A(0);
+  }
+  sum_shares<T, IndexT, kTPR, kSlots>(entries, padded, here, classes, shares, slots, kept, share);
+  const ExpSum<A> own = far_sum<T, kTPR>(in, C, inv_t, slots + 2);
+  const A inv_s = A(1) / own.s;
+#pragma unroll 1
+  for (int64_t col = static_cast<int64_t>(lane) * kVec; col < C; col += kTPR * kVec) {
+    const int n = span_of(C - col, kVec);
+    A v[kVec];
+    load_span<T>(in + col, n, A(0), v);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) v[e] = w * (acc_exp((v[e] - own.m) * inv_t) * inv_s);
+    store_span<T>(out + col, n, v);
+  }
+  group_sync<kTPR>();  // the second store of a listed class comes behind the first
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    if (here[i])
+      IO<T>::store1(out + entries.cls[i], w * (acc_exp((kept[i] - own.m) * inv_t) * inv_s - share[i]));
+  }
+  group_sync<kTPR>();  // the entries' LDS is reused by the next item
+}
+
 // A group of kTPR threads holds a segment of a row, kVPT packets each, and writes its gradient:
 // the softmax everywhere, then the listed classes of the segment again with the teacher's share
 // taken off. The segment is requested before the teacher's side is computed, which hides behind
@@ -473,7 +609,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
   using A = typename IO<T>::Acc;
   using Math = ExpMath<T>;
   constexpr int kVec = IO<T>::kVec, kRows = kSegmentThreads / kTPR;
-  __shared__ A slots[2][kTPR / kWaveSize];
+  __shared__ A slots[4][kTPR / kWaveSize];
   extern __shared__ u32x4 entry_lds[];  // per group: the shares of K entries, then their classes
   const int lane = static_cast<int>(threadIdx.x) % kTPR, group = static_cast<int>(threadIdx.x) / kTPR;
   const int padded = (K + 3) / 4 * 4;
@@ -499,6 +635,15 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
       if (first && lane < cut.head) IO<T>::store1(out + lane, A(0));
       if (first && lane < cut.tail) IO<T>::store1(out + tail_at, A(0));
       for (int64_t p = begin + lane; p < end; p += kTPR) pack_store<T>(out + cut.head + p * kVec, zero);
+      continue;
+    }
+    if (fabs(lse) > A(kFar / 2)) {
+      if (!first) continue;
+      Entries<T, IndexT, kTPR, kSlots> entries;
+      entries.load(row, C, K, inv_t, index, teacher);
+      const A divisor = stats[N];
+      const A w = dl[per_row ? row : 0] * temperature / (divisor > A(0.5) ? divisor : A(0.5));
+      far_row<T, IndexT, kTPR, kSlots>(in, out, C, padded, entries, inv_t, w, classes, shares, slots);
       continue;
     }
     u32x4 raw[kVPT];
@@ -529,46 +674,8 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
       here[i] = cls >= 0 && (edge ? first : cls >= cut.head + begin * kVec && cls < cut.head + end * kVec);
       kept[i] = here[i] ? IO<T>::load1(in + cls) : A(0);
     }
-    const ExpSum<A> t = entries.sum(slots);
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) {
-      const int k = i * kTPR + lane;
-      if (k < padded) {
-        classes[k] = entries.cls[i];
-        shares[k] = entries.cls[i] >= 0 ? acc_exp(entries.z[i] - t.m) / t.s : A(0);
-      }
-      // its logit has arrived before another thread may write over it
-      asm volatile("" : "+v"(kept[i]));
-    }
-    group_sync<kTPR>();
-    // the share of a class is that of every entry of it, four entries at a time
-    bool some = false;
     A share[kSlots];
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) {
-      some |= here[i];
-      share[i] = A(0);
-    }
-    if (some) {
-#pragma unroll 2
-      for (int k = 0; k < padded; k += 4) {
-        int cls[4];
-        A of[4];
-        const u32x4 packed = *reinterpret_cast<const u32x4_any*>(classes + k);
-        cls[0] = packed.x, cls[1] = packed.y, cls[2] = packed.z, cls[3] = packed.w;
-#pragma unroll
-        for (int j = 0; j < 4; j += 16 / static_cast<int>(sizeof(A))) {
-          A part[16 / sizeof(A)];
-          IO<A>::unpack(*reinterpret_cast<const u32x4_any*>(shares + k + j), part);
-#pragma unroll
-          for (int e = 0; e < static_cast<int>(16 / sizeof(A)); ++e) of[j + e] = part[e];
-        }
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) share[i] += cls[j] == entries.cls[i] ? of[j] : A(0);
-      }
-    }
+    sum_shares<T, IndexT, kTPR, kSlots>(entries, padded, here, classes, shares, slots, kept, share);
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) kept[i] = w * (Math::term(kept[i], scale, base) - share[i]);
     if (first && lane < cut.head) IO<T>::store1(out + lane, w * Math::term(head, scale, base));

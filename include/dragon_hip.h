@@ -391,12 +391,16 @@ int dragon_hip_rms_norm_grad(int dtype, int64_t N, int64_t C, const void* h, con
  * nothing is ignored: its loss and gradient are 0 whatever its logits hold, and
  * it is not read. A row whose logits are all -inf, or that holds NaN or +inf,
  * has a NaN loss and NaN gradients.
+ * Loss and gradient hold for logits of any size, rows masked all over by the
+ * type's lowest value among them; rows whose log-sum is beyond +-1024 are read
+ * two times more (the log-sum, a single AccT, no longer holds the sum).
  * normalizer: 0 keeps a loss per row (loss: AccT[N], dl: AccT[N]); otherwise
  * loss = sum of rows / max(divisor, 1) (AccT[1], dl: AccT[1], the gradient
  * divides by max(divisor, 0.5), as ReduceLossGrad) with divisor = normalizer,
  * or the number of rows that are not ignored where normalizer < 0.
  * stats: AccT[N + 1], written by the forward for the backward call: log sum
- * exp(x / t) of each row (+inf for an ignored one), then the divisor (1 for
+ * exp(x / t) of each row (+inf for an ignored one; others are finite, at most
+ * AccT's largest value in size, or NaN), then the divisor (1 for
  * normalizer 0). dx may be the very buffer of x. 1 <= K <= 1024, 1e-18 < t < 1e18,
  * N and C below 2^31. The sums have a fixed order. */
 size_t dragon_hip_topk_distillation_loss_scratch_bytes(int dtype, int64_t N, int64_t C);

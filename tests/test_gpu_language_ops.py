@@ -397,6 +397,62 @@ def test_distillation_masked_vocabulary_empty_rows_and_values_that_are_not_finit
         _check_distill(dtype, xs, index[keep], teacher[keep], 1.0, "VALID", dl[:1], *part)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(6, 130, 3), (6, 4200, 300), (6, 9001, 5), (6, 70001, 9)])
+@pytest.mark.parametrize("temperature", [0.75, 1.0, 1.5, 2.0])
+def test_distillation_of_rows_masked_all_over_and_of_logits_far_from_zero(dtype, shape, temperature):
+    """Loss and gradient depend on differences of logits alone, so the plain form is that of the rows
+    less their largest logit (exact in 64 bits: they are on one grid), with its bounds. Its log-sum is
+    that of the rows less largest / t, two roundings of it and clipped to the type's range."""
+    N, C, k = shape
+    x, index, teacher = _distill_case(N, C, k, dtype, torch.int32, 5, 2.0)
+    g = torch.Generator().manual_seed(3)
+    index.copy_(torch.randint(0, C // 3, (N, k), generator=g))
+    teacher.nan_to_num_(neginf=0.0)
+    low = torch.finfo(x.dtype).min
+    x[0] = low
+    x[1] = low
+    x[1, C // 2:] = -float("inf")
+    x[2] += 30000
+    x[3] -= 30000
+    x[4, C // 3:] = low  # a masked tail: an ordinary row
+    x[5] = low
+    x[5, C - 1] = low / 2  # one class is left, far from zero itself
+    index[5] = C - 1
+    dl = torch.rand(N, generator=g).to(teacher.dtype).cuda()
+    stats, loss, dx = _run_distill(x, index, teacher, temperature, "NONE", dl)
+    a = [L.f64(x), index.cpu().numpy().astype(np.int64), L.f64(teacher)]
+    top = a[0].max(1)
+    top[4] = 0.0
+    with np.errstate(over="ignore"):
+        a[0] -= top[:, None]
+    ws, rows, _ = L.distill_forward(temperature, "NONE", *a)
+    b_lse, b_rows = L.distill_bounds(dtype, temperature, *a)
+    ua = L.u_acc(dtype)
+    most = float(torch.finfo(teacher.dtype).max)
+    with np.errstate(over="ignore"):
+        lse = np.clip(top / temperature + ws[:N], -most, most)
+    L.assert_close(L.f64(stats)[:N], lse, b_lse + 4 * ua * np.abs(lse), "lse")
+    L.assert_close(L.f64(loss), rows, b_rows, "loss")
+    # the ordinary row's gradient is that of its own statistics
+    ws[4] = float(stats[4])
+    want, s, t = L.distill_backward(temperature, "NONE", *a, ws, L.f64(dl))
+    L.assert_close(L.f64(dx), want, L.distill_grad_bound(dtype, temperature, a[0], a[2], a[1], ws, want, s, t), "dx")
+    again = _run_distill(x, index, teacher, temperature, "NONE", dl, in_place=True)
+    assert torch.equal(again[2], dx) and torch.equal(again[0], stats) and torch.equal(again[1], loss)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distillation_of_a_listed_class_that_is_masked_by_the_lowest_value(dtype):
+    N, C, k = 3, 300, 4
+    x, index, teacher = _distill_case(N, C, k, dtype, torch.int64, 8)
+    index.copy_(torch.arange(k).expand(N, k))
+    teacher.copy_(torch.tensor([0.0, 1.0, 2.0, 3.0]).expand(N, k))  # shares of 0.03 to 0.64
+    x[1, 2] = torch.finfo(x.dtype).min
+    dl = torch.ones(N, dtype=teacher.dtype, device="cuda")
+    _check_distill(dtype, x, index, teacher, 1.0, "NONE", dl, *_run_distill(x, index, teacher, 1.0, "NONE", dl))
+
+
 def test_distillation_of_rows_that_list_nothing_and_of_no_rows():
     for N in (0, 3):
         x = torch.randn(N, 100, device="cuda")
