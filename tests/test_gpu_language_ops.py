@@ -442,6 +442,16 @@ def test_distillation_of_rows_masked_all_over_and_of_logits_far_from_zero(dtype,
     assert torch.equal(again[2], dx) and torch.equal(again[0], stats) and torch.equal(again[1], loss)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float64"])
+@pytest.mark.parametrize("N", [1, 2, 15, 16, 17])
+@pytest.mark.parametrize("C,k", [(1000, 40), (2100, 200), (40001, 40), (70000, 200)])
+def test_distillation_reduced_by_the_launch_that_finishes_the_rows(dtype, N, C, k):
+    for reduction in ("VALID", "MEAN", "SUM"):
+        x, index, teacher = _distill_case(N, C, k, dtype, torch.int64, N + k)
+        dl = torch.full((1,), 0.75, dtype=teacher.dtype, device="cuda")
+        _check_distill(dtype, x, index, teacher, 1.5, reduction, dl, *_run_distill(x, index, teacher, 1.5, reduction, dl))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_distillation_of_a_listed_class_that_is_masked_by_the_lowest_value(dtype):
     N, C, k = 3, 300, 4

@@ -106,6 +106,10 @@ def test_plans_by_size():
     assert "IndexT,64,1,true" in plan(f, (2048, 16384, 64)) and "IndexT,256,1,true" in plan(f, (2047, 16384, 64))
     assert "IndexT,256,1,true" in plan(f, (2048, 65536, 64)) and "IndexT,256,1,false" in plan(f, (2048, 65544, 64))
     assert "IndexT,256,1,true" in plan(f, (512, 32768, 64)) and "IndexT,256,1,false" in plan(f, (511, 32768, 64))
+    # up to 16 rows that wavefronts finish are reduced by the same launch
+    assert plan(f, (16, 4096, 64)).count("[") == 1 and plan(f, (17, 4096, 64)).count("[") == 2
+    assert plan(f, (16, 131072, 200)).count("[") == 2 and plan(f, (17, 131072, 200)).count("[") == 3
+    assert plan(f, (16, 131072, 257)).count("[") == 3 and plan(f, (1, 16384, 64)).count("[") == 2
     assert "IndexT,64,1,true" in plan(f, (100, 4096, 64)) and "IndexT,64,4,true" in plan(f, (100, 4096, 256))
     assert "IndexT,256,4,true" in plan(f, (100, 4096, 257)) and "IndexT,256,1,true" in plan(f, (100, 16384, 64))
     assert "IndexT,256,1,false" in plan(f, (100, 16392, 64)) and "distill_forward_join<T,IndexT,64,1>" in plan(f, (100, 16392, 64))
