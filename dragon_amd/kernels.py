@@ -10,6 +10,7 @@ pointers through the C ABI (include/dragon_hip.h) to the gfx950 kernels.
 """
 
 import ctypes
+import threading
 
 import torch
 
@@ -342,6 +343,17 @@ def _raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+class _ThreadScratch(threading.local):
+    """Scratch per (device, stream) of one thread: calls of two threads on one stream may launch
+    their kernels in between each other's."""
+
+    def __init__(self):
+        self.buffers = {}
+
+
+_thread_scratch = _ThreadScratch()
+
+
 def _scratch_for(device, nbytes):
     """Scratch of a call on the current stream. While a graph is being captured it comes from that
     graph's own memory, so that graphs share none and a later, larger call cannot free it."""
@@ -349,9 +361,10 @@ def _scratch_for(device, nbytes):
         return None
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    buf = _scratch.get((device, _raw_stream(device)))
+    buffers, key = _thread_scratch.buffers, (device, _raw_stream(device))
+    buf = buffers.get(key)
     if buf is None or buf.numel() < nbytes:
-        buf = workspace(nbytes, torch.device("cuda", device))
+        buf = buffers[key] = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
     return buf
 
 

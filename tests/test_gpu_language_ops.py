@@ -510,6 +510,45 @@ def test_distillation_offsets_beyond_32_bits():
     assert float(loss[:-2].abs().max()) == 0
 
 
+def test_calls_of_several_threads_on_one_stream():
+    """Each call's launches use scratch that no other thread's call writes in between."""
+    import threading
+    K = _K()
+    cases = []
+    for seed in range(4):
+        x, index, teacher = _distill_case(40, 70001, 20, "float32", torch.int32, seed)
+        h, dy = _make((300, 2048), "float32", seed), _make((300, 2048), "float32", seed + 9)
+        cases.append((x, index, teacher, h, dy, torch.rand(300, device="cuda"), torch.rand(2048, device="cuda")))
+
+    def call(case):
+        x, index, teacher, h, dy, rsig, gamma = case
+        stats, loss = torch.empty(41, device="cuda"), torch.empty(1, device="cuda")
+        K.topk_distillation_loss_forward(40, 70001, 20, 1.0, "MEAN", x, index, teacher, stats, loss)
+        dgamma, dx = torch.empty(2048, device="cuda"), torch.empty_like(h)
+        K.rms_norm_grad(300, 2048, h, rsig, gamma, dy, None, dgamma, dx)
+        return stats, loss, dgamma, dx
+
+    want = [call(c) for c in cases]
+    torch.cuda.synchronize()
+    got, start = [[] for _ in cases], threading.Barrier(len(cases))
+
+    def work(i):
+        start.wait()
+        for _ in range(50):
+            got[i].append(call(cases[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i, calls in enumerate(got):
+        assert len(calls) == 50
+        for outputs in calls:
+            assert all(torch.equal(a, b) for a, b in zip(outputs, want[i]))
+
+
 # ---------------------------------------------------------------- drafted tokens
 
 def _verify_case(B, k, C, dtype, index_dtype, sampled, seed):
