@@ -70,9 +70,28 @@ __device__ __forceinline__ void tile_codes(uint8_t* p, int dup, bool on, float i
   }
 }
 
-// Largest value over `lanes` neighbouring lanes (a power of two, aligned).
-__device__ __forceinline__ float cluster_max(float v, int lanes) {
-  for (int o = 1; o < lanes; o <<= 1) v = MaxOp()(v, __shfl_xor(v, o, kWaveSize));
+// All-reduce over `lanes` neighbouring lanes (4 to 64, a power of two, aligned) by the vector unit's own
+// moves: inside rows of 16 lanes, then the rows' results. Shuffles go through LDS, whose latency the
+// rows wait for: fp32 [13106, 2560] in groups of 128 columns takes 104 us with them, 73 without.
+template <typename Op>
+__device__ __forceinline__ float cluster_reduce(float v, int lanes, Op op) {
+  v = dpp_step<0xB1>(v, op);                    // quad_perm [1,0,3,2]
+  v = dpp_step<0x4E>(v, op);                    // quad_perm [2,3,0,1]
+  if (lanes >= 8) v = dpp_step<0x141>(v, op);   // row_half_mirror
+  if (lanes >= 16) v = dpp_step<0x140>(v, op);  // row_mirror
+  if (lanes >= 32) {
+    auto row = [&](int lane) {
+      return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    };
+    const float low = op(row(0), row(16)), high = op(row(32), row(48));
+    if (lanes == 64) v = op(low, high);
+    else v = (threadIdx.x & 32) ? high : low;
+  }
+  return v;
+}
+template <typename Op>
+__device__ __forceinline__ double cluster_reduce(double v, int lanes, Op op) {
+  for (int o = 1; o < lanes; o <<= 1) v = op(v, __shfl_xor(v, o, kWaveSize));
   return v;
 }
 
@@ -154,7 +173,7 @@ __global__ __launch_bounds__(kLoopThreads) void rms_norm_rows_looped(
           top = 0.f;
 #pragma unroll
           for (int e = 0; e < kVec; ++e) top = MaxOp()(top, fabsf(v[e]));
-          top = MaxOp()(cluster_max(top, group / kVec), kAmaxFloor);
+          top = MaxOp()(cluster_reduce(top, group / kVec, MaxOp()), kAmaxFloor);
           if (on && col % group == 0) scale[row * groups + col / group] = top / kFp8Max;
         }
         const float inv = kFp8Max / top;
@@ -237,9 +256,7 @@ struct RowPackets {
 template <int kTPR, typename A, typename Op>
 __device__ __forceinline__ A row_allreduce(A v, Op op, A* slots) {
   if constexpr (kTPR < kWaveSize) {
-#pragma unroll
-    for (int o = kTPR / 2; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, kWaveSize));
-    return v;
+    return cluster_reduce(v, kTPR, op);
   } else {
     v = wave_allreduce(v, op);
     if constexpr (kTPR == kWaveSize) return v;
@@ -329,7 +346,7 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
         } else {
           // a group wider than the row stays inside the row's own lanes
           const int lanes = group / kVec < kTPR ? group / kVec : kTPR;
-          const float amax = MaxOp()(cluster_max(part, lanes), kAmaxFloor);
+          const float amax = MaxOp()(cluster_reduce(part, lanes, MaxOp()), kAmaxFloor);
           const int nominal = tile.col[s] + tile.dup[s];
           if (valid && tile.on[s] && nominal % group == 0) scale[row * groups + nominal / group] = amax / kFp8Max;
           tile_codes<kRagged>(q + row * C + tile.col[s], tile.dup[s], valid && tile.on[s], kFp8Max / amax, v[s]);
@@ -353,7 +370,10 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
 }
 
 // Calls LAUNCH(threads per row, packets per thread) for rows of `packets`: the fewest threads
-// that hold the row with up to two packets each, four on the largest workgroup.
+// that hold the row with up to two packets each, four on the largest workgroup. Powers of two up to 512
+// threads, where half-empty slots cost next to nothing (steps of a wavefront: bf16 [13106, 5120] 88.7 us
+// against 89.1); beyond them bf16 [7280, 9216] takes 94.5 us by 1024 threads, 89.6 by 640, with e4m3
+// codes 86.0 and 77.0.
 #define DRAGON_HIP_RMS_SWITCH_2(packets, LAUNCH)  \
   if (packets <= 8) LAUNCH(8, 1)                  \
   else if (packets <= 16) LAUNCH(16, 1)           \
@@ -363,6 +383,8 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
   else if (packets <= 256) LAUNCH(128, 2)         \
   else if (packets <= 512) LAUNCH(256, 2)         \
   else if (packets <= 1024) LAUNCH(512, 2)        \
+  else if (packets <= 1280) LAUNCH(640, 2)        \
+  else if (packets <= 1536) LAUNCH(768, 2)        \
   else LAUNCH(1024, 2)
 #define DRAGON_HIP_RMS_SWITCH(packets, LAUNCH) \
   if (packets > 2048) LAUNCH(1024, 4)          \
@@ -374,8 +396,10 @@ constexpr int64_t kMaxTilePackets = 4096;
 // twenty-four): bf16 [8192, 8192] with a residual 109 us at four, 91 at eight, 92 at twenty-four, 99
 // with a workgroup per row; its gradient at [8192, 4096] 49 us at eight, 53 at sixteen, 58 at
 // thirty-two. More streams at a time are further apart in memory, and leave more partial sums.
-// Quantised rows that are not whole packets, which compute more per byte, take twice as many:
-// fp16 [19870, 805] in groups of 128 columns 25.0 us at eight, 22.7 at sixteen.
+// Quantised rows compute more per byte and wait for more reductions; those that leave some of the tile's
+// slots empty, or are not whole packets, take twice as many in workgroups of up to 512 threads: in groups
+// of 128 columns bf16 [58254, 1152] 95.9 us at eight, 82.4 at sixteen, [9362, 7168] 85.7 and 77.7,
+// [10922, 6144] 73.8 and 76.3; full rows lose by it ([16384, 4096] 75.3 and 78.2).
 inline int64_t rms_grid(int threads) {
   return static_cast<int64_t>(num_cus()) * (threads < 512 ? 512 / threads : 1);
 }
@@ -387,7 +411,8 @@ int launch_rms_tile(int64_t N, int64_t C, float eps, const void* x, const void* 
   using A = typename IO<T>::Acc;
   constexpr int kThreads = tile_threads(kTPR);
   const int64_t want = ceil_div(N, kThreads / kTPR);
-  const int64_t most = rms_grid(kThreads) * (kRagged && kOut != kPlain ? 2 : 1);
+  const bool more = kOut != kPlain && kThreads <= 512 && (kRagged || ceil_div(C, IO<T>::kVec) < kTPR * kVPT);
+  const int64_t most = rms_grid(kThreads) * (more ? 2 : 1);
   note_number("threads_per_row", kTPR);
   note_number("packets", kVPT);
   hipLaunchKernelGGL((rms_norm_rows<T, kTPR, kVPT, kRagged, kResidual, kOut>),
@@ -553,7 +578,7 @@ __global__ __launch_bounds__(kColThreads) void rms_norm_grad_cols(
 // One read of h, dy and dh, one write of dx, and the column sums in the registers of workgroups
 // that stay and walk the rows: a thread owns the same columns of every row it meets. The groups
 // of a workgroup add theirs in LDS, in order, and each workgroup leaves one row of partial sums.
-constexpr int grad_threads(int tpr) { return tpr <= 512 ? 512 : 1024; }
+constexpr int grad_threads(int tpr) { return tpr <= 512 ? 512 : tpr; }
 template <typename T, int kTPR, int kVPT, bool kRagged, bool kThrough>
 __global__ __launch_bounds__(grad_threads(kTPR)) void rms_norm_grad_rows(
     const int64_t N, const int C, const T* h, const typename IO<T>::Acc* rsig,

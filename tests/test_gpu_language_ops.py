@@ -857,6 +857,31 @@ def test_rms_norm_at_the_seams(dtype, vec):
 
 
 @pytest.mark.parametrize("dtype,vec", [("bfloat16", 8), ("float32", 4)])
+@pytest.mark.parametrize("packets", [40, 144, 320, 896, 1025, 1279, 1280, 1281, 1535, 1536, 1537])
+def test_rms_norm_of_rows_that_leave_slots_empty(dtype, vec, packets):
+    """Tiles of 640 and 768 threads and those beside them; rows more than the workgroups, so that they walk."""
+    K = _K()
+    for C, N in ((packets * vec, 1100), (packets * vec - 1, 5), (packets * vec + 1, 530)):
+        x, r, dy = (_make((N, C), dtype, packets + i) for i in range(3))
+        gamma = (1 + _make((C,), "float64", 9, 0.3)).float()
+        h, y, rsig = torch.empty_like(x), torch.empty_like(x), torch.empty(N, device="cuda")
+        K.rms_norm(N, C, 1e-5, x, r, gamma, h, rsig, y)
+        s, rs, want = L.rms_norm(L.f64(x), L.f64(r), L.f64(gamma), float(np.float32(1e-5)))
+        bh, brs, by = L.rms_norm_bounds(dtype, s, rs, want)
+        L.assert_close(L.f64(h), s, bh, "h %d" % C)
+        L.assert_close(L.f64(rsig), rs, brs, "rsig %d" % C)
+        L.assert_close(L.f64(y), want, by, "y %d" % C)
+        dgamma, dx = torch.empty_like(gamma), torch.empty_like(x)
+        K.rms_norm_grad(N, C, h, rsig, gamma, dy, r, dgamma, dx)
+        _check_grad(dtype, h, rsig, gamma, dy, r, dgamma, dx)
+        for group in (0, 32, 128, 256):
+            q = torch.empty((N, C), dtype=torch.float8_e4m3fn, device="cuda")
+            scale = torch.empty((N, -(-C // group) if group else 1), device="cuda")
+            K.rms_norm_quant(N, C, group, 1e-5, x, r, gamma, h, rsig, q, scale)
+            _check_quant(dtype, group, x, r, gamma, h, rsig, q, scale)
+
+
+@pytest.mark.parametrize("dtype,vec", [("bfloat16", 8), ("float32", 4)])
 def test_distillation_at_the_seams(dtype, vec):
     for packets in (256, 512, 1024, 2048, 2600):
         for extra in (-1, 0, 1):

@@ -98,6 +98,9 @@ def test_plans_by_size():
     assert plan("rms_norm", (8, 4096)).startswith("threads_per_row=256:packets=2:rms_norm_rows<")
     assert plan("rms_norm", (8, 64)).startswith("threads_per_row=8:packets=1:")
     assert plan("rms_norm", (8, 32768)).startswith("threads_per_row=1024:packets=4:")
+    for columns, threads in ((8192, 512), (8200, 640), (10240, 640), (10248, 768), (12288, 768), (12296, 1024)):
+        assert plan("rms_norm", (8, columns)).startswith("threads_per_row=%d:packets=2:" % threads)
+        assert "grad_rows<T,%d,2" % threads in plan("rms_norm_grad", (8, columns))
     assert "rms_norm_rows_looped" in plan("rms_norm", (8, 32769)) and "looped" in plan("rms_norm", (8, 7))
     assert "rms_norm_rows_looped" in plan("rms_norm_quant", (8, 40000, 128))
     assert "grad_rows" in plan("rms_norm_grad", (8, 16384)) and "grad_dots" in plan("rms_norm_grad", (8, 16392))
