@@ -49,21 +49,21 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int n, const float (&v)[
   }
 }
 
-// The codes of a tile's packet, v times `inv`. The packet that was moved back writes only the
-// elements that are its own: those before may belong to a group of another scale.
+// The codes of a tile's packet, v times `inv`, but for the first `skip`: those of a packet that was
+// moved back into a group of another scale.
 template <bool kRagged, int kVec>
-__device__ __forceinline__ void tile_codes(uint8_t* p, int dup, bool on, float inv, const float (&v)[kVec]) {
+__device__ __forceinline__ void tile_codes(uint8_t* p, int skip, bool on, float inv, const float (&v)[kVec]) {
   float w[kVec];
 #pragma unroll
   for (int e = 0; e < kVec; ++e) w[e] = v[e] * inv;
   if (!on) return;
-  if (kRagged && dup > 0) {
+  if (kRagged && skip > 0) {
     const uint32_t lo = e4m3x4(w[0], w[1], w[2], w[3]);
     uint32_t hi = 0;
     if constexpr (kVec == 8) hi = e4m3x4(w[4], w[5], w[6], w[7]);
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
-      if (e >= dup) p[e] = static_cast<uint8_t>((e < 4 ? lo : hi) >> (8 * (e & 3)));
+      if (e >= skip) p[e] = static_cast<uint8_t>((e < 4 ? lo : hi) >> (8 * (e & 3)));
     }
   } else {
     store_codes<kVec>(p, kVec, w);
@@ -348,8 +348,9 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
           const int lanes = group / kVec < kTPR ? group / kVec : kTPR;
           const float amax = MaxOp()(cluster_reduce(part, lanes, MaxOp()), kAmaxFloor);
           const int nominal = tile.col[s] + tile.dup[s];
-          if (valid && tile.on[s] && nominal % group == 0) scale[row * groups + nominal / group] = amax / kFp8Max;
-          tile_codes<kRagged>(q + row * C + tile.col[s], tile.dup[s], valid && tile.on[s], kFp8Max / amax, v[s]);
+          const bool leads = nominal % group == 0;  // its group
+          if (valid && tile.on[s] && leads) scale[row * groups + nominal / group] = amax / kFp8Max;
+          tile_codes<kRagged>(q + row * C + tile.col[s], leads ? tile.dup[s] : 0, valid && tile.on[s], kFp8Max / amax, v[s]);
         }
       }
     }
@@ -358,7 +359,7 @@ __global__ __launch_bounds__(tile_threads(kTPR)) void rms_norm_rows(
       if (valid && threadIdx.x % kTPR == 0) scale[row] = amax / kFp8Max;
 #pragma unroll
       for (int s = 0; s < kVPT; ++s)
-        tile_codes<kRagged>(q + row * C + tile.col[s], tile.dup[s], valid && tile.on[s], kFp8Max / amax, v[s]);
+        tile_codes<kRagged>(q + row * C + tile.col[s], 0, valid && tile.on[s], kFp8Max / amax, v[s]);
     }
     row = next;
     turn ^= 1;
@@ -396,10 +397,11 @@ constexpr int64_t kMaxTilePackets = 4096;
 // twenty-four): bf16 [8192, 8192] with a residual 109 us at four, 91 at eight, 92 at twenty-four, 99
 // with a workgroup per row; its gradient at [8192, 4096] 49 us at eight, 53 at sixteen, 58 at
 // thirty-two. More streams at a time are further apart in memory, and leave more partial sums.
-// Quantised rows compute more per byte and wait for more reductions; those that leave some of the tile's
-// slots empty, or are not whole packets, take twice as many in workgroups of up to 512 threads: in groups
-// of 128 columns bf16 [58254, 1152] 95.9 us at eight, 82.4 at sixteen, [9362, 7168] 85.7 and 77.7,
-// [10922, 6144] 73.8 and 76.3; full rows lose by it ([16384, 4096] 75.3 and 78.2).
+// Quantised rows compute more per byte and wait for more reductions; those that leave a sixteenth of the
+// tile's slots and more empty take twice as many, in workgroups of up to 512 threads: in groups of 128
+// columns bf16 [58254, 1152] 95.9 us at eight, 82.4 at sixteen, [9362, 7168] 85.7 and 77.7, [10922, 6144]
+// 73.8 and 76.3; fuller rows lose by it (bf16 [16384, 4096] 75.3 and 78.2, fp32 [33520, 1001] 78.6 and
+// 87.5), and rows that are not quantised (bf16 [29127, 1152] 90.2 and 101.7).
 inline int64_t rms_grid(int threads) {
   return static_cast<int64_t>(num_cus()) * (threads < 512 ? 512 / threads : 1);
 }
@@ -411,7 +413,7 @@ int launch_rms_tile(int64_t N, int64_t C, float eps, const void* x, const void* 
   using A = typename IO<T>::Acc;
   constexpr int kThreads = tile_threads(kTPR);
   const int64_t want = ceil_div(N, kThreads / kTPR);
-  const bool more = kOut != kPlain && kThreads <= 512 && (kRagged || ceil_div(C, IO<T>::kVec) < kTPR * kVPT);
+  const bool more = kOut != kPlain && kThreads <= 512 && ceil_div(C, IO<T>::kVec) * 16 < kTPR * kVPT * 15;
   const int64_t most = rms_grid(kThreads) * (more ? 2 : 1);
   note_number("threads_per_row", kTPR);
   note_number("packets", kVPT);
