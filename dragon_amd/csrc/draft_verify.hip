@@ -517,7 +517,10 @@ int dragon_hip_draft_verify(int dtype, int index_dtype, int64_t B, int64_t K, in
   if (!target || !u_sample || !tokens || !accepted || (K > 0 && (!drafted || !u_accept)))
     return DRAGON_HIP_EINVAL;
   // several workgroups read the inputs of a sequence whose outputs one of them writes
-  if (accepted == lengths || accepted == drafted || tokens == drafted || tokens == lengths || tokens == accepted)
+  const uint64_t one = index_dtype == DRAGON_HIP_I32 ? 4 : 8, each = B * one, all = each * K;
+  if (overlaps(accepted, each, lengths, each) || overlaps(accepted, each, drafted, all) ||
+      overlaps(tokens, all + each, drafted, all) || overlaps(tokens, all + each, lengths, each) ||
+      overlaps(tokens, all + each, accepted, each))
     return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_DTYPE(dtype, launch_verify_index, index_dtype, B, K, C, target, draft, drafted,

@@ -12,7 +12,7 @@ namespace dragon_hip {
 namespace {
 
 // Distinct, aligned, never dereferenced.
-inline void* fake(int k) { return reinterpret_cast<void*>(static_cast<uintptr_t>(0x100000000ull) * (k + 1)); }
+inline void* fake(int k) { return reinterpret_cast<void*>(static_cast<uintptr_t>(0x10000000000ull) * (k + 1)); }
 
 struct PlanScope {
   PlanScope() {

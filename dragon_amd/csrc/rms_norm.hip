@@ -871,6 +871,9 @@ int launch_rms_norm_grad(int64_t N, int64_t C, const void* h, const void* rsig, 
   return status_of_launch();
 }
 
+inline int element_bytes(int dtype) {
+  return dtype == DRAGON_HIP_F64 ? 8 : (dtype == DRAGON_HIP_F32 ? 4 : 2);
+}
 inline bool sizes_ok(int64_t N, int64_t C) { return N >= 0 && C > 0 && N <= INT_MAX && C <= INT_MAX; }
 
 } // namespace
@@ -885,7 +888,10 @@ int dragon_hip_rms_norm(int dtype, int64_t N, int64_t C, float eps, const void* 
                         void* stream) {
   if (!sizes_ok(N, C)) return DRAGON_HIP_EINVAL;
   if (N == 0) return DRAGON_HIP_OK;
-  if (!x || !gamma || !y || y == h) return DRAGON_HIP_EINVAL;
+  const uint64_t bytes = static_cast<uint64_t>(N) * C * element_bytes(dtype);
+  if (!x || !gamma || !y || overlaps(y, bytes, h, bytes)) return DRAGON_HIP_EINVAL;
+  if (across(y, x, bytes) || across(y, residual, bytes) || across(h, x, bytes) || across(h, residual, bytes))
+    return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_DTYPE(dtype, launch_rms_norm, N, C, eps, x, residual, gamma, h, rsig, y, s);
 }
@@ -899,6 +905,10 @@ int dragon_hip_rms_norm_quant(int dtype, int64_t N, int64_t C, int64_t group, fl
   if (group != 0 && group != 32 && group != 64 && group != 128 && group != 256) return DRAGON_HIP_EINVAL;
   if (N == 0) return DRAGON_HIP_OK;
   if (!x || !gamma || !q || !scale) return DRAGON_HIP_EINVAL;
+  const uint64_t codes = static_cast<uint64_t>(N) * C, bytes = codes * element_bytes(dtype);
+  if (across(h, x, bytes) || across(h, residual, bytes) || overlaps(q, codes, x, bytes) ||
+      overlaps(q, codes, residual, bytes) || overlaps(q, codes, h, bytes))
+    return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case DRAGON_HIP_F16:
@@ -925,7 +935,10 @@ int dragon_hip_rms_norm_grad(int dtype, int64_t N, int64_t C, const void* h, con
                              const void* gamma, const void* dy, const void* dh, void* dgamma,
                              void* dx, void* scratch, size_t scratch_bytes, void* stream) {
   if (!sizes_ok(N, C)) return DRAGON_HIP_EINVAL;
-  if (!dgamma || (N > 0 && (!h || !rsig || !gamma || !dy || !dx || dx == h))) return DRAGON_HIP_EINVAL;
+  if (!dgamma || (N > 0 && (!h || !rsig || !gamma || !dy || !dx))) return DRAGON_HIP_EINVAL;
+  const uint64_t bytes = static_cast<uint64_t>(N) * C * element_bytes(dtype);
+  if (N > 0 && (overlaps(dx, bytes, h, bytes) || across(dx, dy, bytes) || across(dx, dh, bytes)))
+    return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_DTYPE(dtype, launch_rms_norm_grad, N, C, h, rsig, gamma, dy, dh, dgamma, dx,
                             scratch, scratch_bytes, s);

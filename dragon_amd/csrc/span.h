@@ -1,5 +1,6 @@
 // Pieces of rows at any alignment, shared by the kernels that walk rows packet
-// by packet: up to kVec elements from an element-aligned address.
+// by packet: up to kVec elements from an element-aligned address. And the host's
+// check that an output does not lie across a tensor.
 #pragma once
 
 #include "common.h"
@@ -35,6 +36,16 @@ __device__ __forceinline__ void store_span(T* p, int n, const typename IO<T>::Ac
       if (e < n) IO<T>::store1(p + e, v[e]);
     }
   }
+}
+
+// Whether two tensors of so many bytes share memory; a null pointer is no tensor.
+inline bool overlaps(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  return p && q && p < q + b_bytes && q < p + a_bytes;
+}
+// Whether an output shares memory with an input of its size without being the very buffer of it.
+inline bool across(const void* out, const void* in, uint64_t bytes) {
+  return out != in && overlaps(out, bytes, in, bytes);
 }
 
 } // namespace dragon_hip

@@ -841,6 +841,8 @@ int dragon_hip_topk_distillation_loss_backward(int dtype, int index_dtype, int64
   if (!sizes_ok(N, C, K, temperature, normalizer)) return DRAGON_HIP_EINVAL;
   if (N == 0) return DRAGON_HIP_OK;
   if (!x || !index || !teacher || !stats || !dl || !dx) return DRAGON_HIP_EINVAL;
+  const int element = dtype == DRAGON_HIP_F64 ? 8 : (dtype == DRAGON_HIP_F32 ? 4 : 2);
+  if (across(dx, x, static_cast<uint64_t>(N) * C * element)) return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_INDEXED(dtype, index_dtype, launch_backward, N, C, K, temperature, normalizer, x,
                               index, teacher, stats, dl, dx, s);

@@ -352,7 +352,8 @@ int dragon_hip_softmax_cross_entropy_loss_backward(int dtype, int target_dtype, 
  * x, residual, y, h: T[N, C]; gamma: AccT[C]; rsig: AccT[N]. s is held in AccT
  * and rounded once into h and once into y. h and rsig may be NULL where the
  * caller has no use for them. Each output may be the very buffer of x or of
- * residual (y and h may not be the same buffer). N and C below 2^31. */
+ * residual (y and h may not be the same buffer); memory shared in any other way
+ * is refused, here and in the calls below. N and C below 2^31. */
 int dragon_hip_rms_norm(int dtype, int64_t N, int64_t C, float eps, const void* x,
                         const void* residual, const void* gamma, void* h, void* rsig, void* y,
                         void* stream);
@@ -361,7 +362,7 @@ int dragon_hip_rms_norm(int dtype, int64_t N, int64_t C, float eps, const void* 
  * consecutive columns of a row (32, 64, 128 or 256; 0: the whole row is one
  * group; the last group of a row may be shorter):
  *   scale = max(max|y|, 1e-30) / 448,  q = e4m3(y / scale)
- * q: one byte per element [N, C]; scale: float[N, ceil(C / group)]. A NaN in y
+ * q: one byte per element [N, C], apart from x, residual and h; scale: float[N, ceil(C / group)]. A NaN in y
  * becomes a NaN code and is passed over by the maximum; an infinity makes its
  * group's scale infinite. dtype F16, BF16 or F32 (DRAGON_HIP_EDTYPE otherwise). */
 int dragon_hip_rms_norm_quant(int dtype, int64_t N, int64_t C, int64_t group, float eps,

@@ -52,6 +52,31 @@ def test_rms_norm_grad_refusals():
     assert lib.dragon_hip_rms_norm_grad_scratch_bytes(7, 4, 8) == 0
 
 
+def test_outputs_that_lie_across_inputs_are_refused():
+    """Shifted by one element, or of another width: whatever is read after it is written would be lost."""
+    lib = _lib.lib()
+    at = lambda p, shift: ctypes.c_void_p(p.value + shift)
+    norm = lambda x=P[0], r=P[1], h=P[3], y=P[5]: lib.dragon_hip_rms_norm(1, 4, 8, 1e-5, x, r, P[2], h, P[4], y, None)
+    for shift in (2, -2, 62, -62):
+        assert norm(y=at(P[0], shift)) == EINVAL and norm(y=at(P[1], shift)) == EINVAL
+        assert norm(h=at(P[0], shift)) == EINVAL and norm(h=at(P[1], shift)) == EINVAL
+        assert norm(y=at(P[3], shift)) == EINVAL
+    quant = lambda h=P[3], q=P[5]: lib.dragon_hip_rms_norm_quant(1, 4, 8, 0, 1e-5, P[0], P[1], P[2], h, P[4], q, P[6], None)
+    for other in (P[0], P[1], P[3]):
+        assert quant(q=other) == EINVAL and quant(q=at(other, 63)) == EINVAL and quant(q=at(other, -31)) == EINVAL
+    assert quant(h=at(P[0], 4)) == EINVAL
+    grad = lambda dx: lib.dragon_hip_rms_norm_grad(2, 4, 8, P[0], P[1], P[2], P[3], P[4], P[5], dx, P[7], BIG, None)
+    for shift in (4, -4, 124):
+        assert grad(at(P[0], shift)) == EINVAL and grad(at(P[3], shift)) == EINVAL and grad(at(P[4], shift)) == EINVAL
+    loss = lambda dx: lib.dragon_hip_topk_distillation_loss_backward(3, 5, 4, 8, 2, 1.0, -1.0, P[0], P[1], P[2], P[3], P[4],
+                                                                     dx, None)
+    assert loss(at(P[0], 8)) == EINVAL and loss(at(P[0], -248)) == EINVAL
+    verify = lambda tok=P[6], acc=P[7]: lib.dragon_hip_draft_verify(2, 5, 2, 3, 8, P[0], P[1], P[2], P[3], P[4], P[5], tok, acc,
+                                                                    P[8], BIG, None)
+    assert verify(tok=at(P[2], 40)) == EINVAL and verify(tok=at(P[2], -56)) == EINVAL and verify(tok=at(P[3], -8)) == EINVAL
+    assert verify(acc=at(P[2], 8)) == EINVAL and verify(acc=at(P[6], 56)) == EINVAL
+
+
 def test_distillation_refusals():
     lib = _lib.lib()
     fwd = lambda dtype=1, it=5, N=4, C=8, k=2, t=1.0, norm=-1.0, x=P[0], st=P[3], loss=P[4], ws=P[5], nbytes=BIG: \
