@@ -31,15 +31,15 @@ __device__ __forceinline__ int64_t length_of(const IndexT* lengths, int64_t b, i
 }
 
 // How many of a sequence's drafted tokens pass, and how many there are. Found by one wavefront, 64
-// positions at a time: the first lane that refuses ends it. What a position is judged by is
+// positions at a time: the first lane that refuses ends it. What a position is decided by is
 // requested beside the length, not behind it.
-struct Verdict {
+struct Prefix {
   int64_t n, len;
 };
 template <typename T, typename IndexT>
-__device__ __forceinline__ Verdict judge(const int64_t b, const int64_t K, const int64_t C, const T* target,
-                                         const T* draft, const IndexT* drafted, const IndexT* lengths,
-                                         const float* u_accept) {
+__device__ __forceinline__ Prefix accepted_prefix(const int64_t b, const int64_t K, const int64_t C,
+                                                  const T* target, const T* draft, const IndexT* drafted,
+                                                  const IndexT* lengths, const float* u_accept) {
   const int lane = threadIdx.x & (kWaveSize - 1);
   int64_t len = K;
   for (int64_t first = 0; first < K; first += kWaveSize) {
@@ -319,7 +319,7 @@ __device__ __forceinline__ int64_t pick_class(SampleRow<T> row, const int64_t C,
 }
 
 template <typename T, typename IndexT>
-__device__ __forceinline__ SampleRow<T> sample_row(int64_t b, int64_t K, int64_t C, const Verdict& v,
+__device__ __forceinline__ SampleRow<T> sample_row(int64_t b, int64_t K, int64_t C, const Prefix& v,
                                                    const T* target, const T* draft, const IndexT* drafted) {
   SampleRow<T> row = {target + (b * (K + 1) + v.n) * C, nullptr, -1};
   if (v.n < v.len) {
@@ -343,16 +343,16 @@ __global__ __launch_bounds__(rows_waves<T>() * kWaveSize) void draft_verify_rows
     IndexT* __restrict__ accepted) {
   constexpr int kRowsWaves = rows_waves<T>();
   __shared__ double runs[kMaxRuns];
-  __shared__ Verdict verdict;
+  __shared__ Prefix prefix;
   const int lane = threadIdx.x & (kWaveSize - 1);
   for (int64_t b = blockIdx.x; b < B; b += gridDim.x) {
     const float u = u_sample[b];
     if (threadIdx.x < kWaveSize) {
-      const Verdict v = judge(b, K, C, target, draft, drafted, lengths, u_accept);
-      if (threadIdx.x == 0) verdict = v;
+      const Prefix v = accepted_prefix(b, K, C, target, draft, drafted, lengths, u_accept);
+      if (threadIdx.x == 0) prefix = v;
     }
     __syncthreads();
-    const Verdict v = verdict;
+    const Prefix v = prefix;
     const SampleRow<T> row = sample_row(b, K, C, v, target, draft, drafted);
     sum_runs<kRowsWaves, 2>(row, 0, C, [&](int64_t run, double sum) {
       if (lane == 0 && run < kMaxRuns) runs[run] = sum;
@@ -379,19 +379,19 @@ __global__ __launch_bounds__(kPartWaves * kWaveSize) void draft_verify_runs(
     const int64_t row_runs, const T* __restrict__ target, const T* __restrict__ draft,
     const IndexT* __restrict__ drafted, const IndexT* __restrict__ lengths,
     const float* __restrict__ u_accept, IndexT* __restrict__ accepted, double* __restrict__ sums) {
-  __shared__ Verdict verdict;
+  __shared__ Prefix prefix;
   const int lane = threadIdx.x & (kWaveSize - 1);
   for (int64_t item = blockIdx.x; item < B * parts; item += gridDim.x) {
     const int64_t b = item / parts, part = item - b * parts;
     if (threadIdx.x < kWaveSize) {
-      const Verdict v = judge(b, K, C, target, draft, drafted, lengths, u_accept);
+      const Prefix v = accepted_prefix(b, K, C, target, draft, drafted, lengths, u_accept);
       if (threadIdx.x == 0) {
-        verdict = v;
+        prefix = v;
         if (part == 0) accepted[b] = static_cast<IndexT>(v.n);
       }
     }
     __syncthreads();
-    const SampleRow<T> row = sample_row(b, K, C, verdict, target, draft, drafted);
+    const SampleRow<T> row = sample_row(b, K, C, prefix, target, draft, drafted);
     const int64_t first = part * part_runs, last = first + part_runs < row_runs ? first + part_runs : row_runs;
     const int64_t begin = first * run_classes<T>();
     const int64_t end = last * run_classes<T>() < C ? last * run_classes<T>() : C;
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(kPartWaves * kWaveSize) void draft_verify_runs(
     sum_runs<kPartWaves, IO<T>::kVec == 8 ? 2 : 4>(row, begin, end, [&](int64_t run, double sum) {
       if (lane == 0 && first + run < last) out[run] = sum;
     });
-    __syncthreads();  // the verdict is overwritten by the next item's
+    __syncthreads();  // the prefix is overwritten by the next item's
   }
 }
 template <typename T, typename IndexT>
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(kPartWaves * kWaveSize) void draft_verify_pick(
     const float* __restrict__ u_sample, IndexT* __restrict__ tokens, const IndexT* __restrict__ accepted,
     double* __restrict__ sums) {
   for (int64_t b = blockIdx.x; b < B; b += gridDim.x) {
-    const Verdict v = {static_cast<int64_t>(accepted[b]), length_of(lengths, b, K)};
+    const Prefix v = {static_cast<int64_t>(accepted[b]), length_of(lengths, b, K)};
     const SampleRow<T> row = sample_row(b, K, C, v, target, draft, drafted);
     const int64_t token = pick_class<kPartWaves>(row, C, row_runs, sums + b * row_runs, u_sample[b]);
     if (threadIdx.x == 0) tokens[b * (K + 1) + v.n] = static_cast<IndexT>(token);
