@@ -176,9 +176,8 @@ struct Entries {
   using A = typename IO<T>::Acc;
   static constexpr int kSlots = kSlotsT;
   int cls[kSlots];  // -1: not listed
-  A z[kSlots];      // teacher's logit / t
-  __device__ __forceinline__ void load(int64_t row, int64_t C, int K, A inv_t, const IndexT* index,
-                                       const A* teacher) {
+  A z[kSlots];      // teacher's logit, -inf where it is not listed
+  __device__ __forceinline__ void load(int64_t row, int64_t C, int K, const IndexT* index, const A* teacher) {
     const int lane = static_cast<int>(threadIdx.x) % kTPR;
     IndexT c[kSlots];
     A l[kSlots];
@@ -195,7 +194,7 @@ struct Entries {
     for (int i = 0; i < kSlots; ++i) {
       const bool listed = c[i] >= 0 && static_cast<int64_t>(c[i]) < C && l[i] != acc_neg_inf<A>();
       cls[i] = listed ? static_cast<int>(c[i]) : -1;
-      z[i] = listed ? l[i] * inv_t : acc_neg_inf<A>();
+      z[i] = listed ? l[i] : acc_neg_inf<A>();
     }
   }
   __device__ __forceinline__ bool any() const {
@@ -204,15 +203,19 @@ struct Entries {
     for (int i = 0; i < kSlots; ++i) on |= cls[i] >= 0;
     return group_any<kTPR>(on);
   }
+  // How far entry i lies below the maximum m, at the temperature. The difference comes first: a quotient of
+  // its own would be rounded relative to the logit, not to the difference that decides the share (parts in 10^3
+  // of it at 30000), and the type's lowest value has none at t < 1.
+  __device__ __forceinline__ A offset(int i, A m, A inv_t) const { return (z[i] - m) * inv_t; }
   // Their maximum (which passes over NaN) and the sum of their exponentials (which keeps it).
-  __device__ __forceinline__ ExpSum<A> sum(A (*slots)[kTPR / kWaveSize]) const {
+  __device__ __forceinline__ ExpSum<A> sum(A inv_t, A (*slots)[kTPR / kWaveSize]) const {
     A m = acc_neg_inf<A>();
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) m = MaxOp()(m, z[i]);
     m = group_reduce<kTPR>(m, MaxOp(), slots[0]);
     A total = A(0);
 #pragma unroll
-    for (int i = 0; i < kSlots; ++i) total += cls[i] >= 0 ? acc_exp(z[i] - m) : A(0);
+    for (int i = 0; i < kSlots; ++i) total += cls[i] >= 0 ? acc_exp(offset(i, m, inv_t)) : A(0);
     return {m, group_reduce<kTPR>(total, SumOp(), slots[1])};
   }
 };
@@ -232,7 +235,7 @@ __device__ __forceinline__ typename IO<T>::Acc finish_row(const int64_t row, con
 #pragma unroll
   for (int i = 0; i < kSlots; ++i)
     xk[i] = entries.cls[i] >= 0 ? IO<T>::load1(x + row * C + entries.cls[i]) : A(0);
-  const ExpSum<A> t = entries.sum(slots);
+  const ExpSum<A> t = entries.sum(inv_t, slots);
   const A log_total = acc_log(t.s);
   const A scale = ExpMath<T>::scale(inv_t);
   A log_s = acc_log(run.s), lse = ExpMath<T>::log_of(run.m, run.s);
@@ -251,7 +254,7 @@ __device__ __forceinline__ typename IO<T>::Acc finish_row(const int64_t row, con
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
     if (entries.cls[i] < 0) continue;
-    const A log_p = entries.z[i] - t.m - log_total;
+    const A log_p = entries.offset(i, t.m, inv_t) - log_total;
     const A p = acc_exp(log_p);
     const A below = far ? (largest - xk[i]) * inv_t : ExpMath<T>::below(xk[i], scale, run.m);
     if (p != A(0)) part += p * (log_p + (below + log_s));
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(row_threads(kReduce)) void distill_forward_segments
     const int64_t row = kWhole ? item : item / segments;
     const uint32_t segment = kWhole ? 0 : static_cast<uint32_t>(item - row * segments);
     Entries<T, IndexT, kTPR, kSlots> entries;
-    entries.load(row, C, K, inv_t, index, teacher);
+    entries.load(row, C, K, index, teacher);
     if (!entries.any()) {
       if (lane == 0 && segment == 0) {
         stats[row] = -acc_neg_inf<A>();
@@ -396,7 +399,7 @@ __global__ __launch_bounds__(row_threads(kReduce)) void distill_forward_join(
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTPR; row < N;
        row += static_cast<int64_t>(gridDim.x) * kRows) {
     Entries<T, IndexT, kTPR, kSlots> entries;
-    entries.load(row, C, K, inv_t, index, teacher);
+    entries.load(row, C, K, index, teacher);
     if (!entries.any()) continue;  // written by the row's first segment, which left no pair
     ExpSum<A> run = ExpSum<A>::none();
     for (int i = lane; i < segments; i += kTPR) {
@@ -545,7 +548,8 @@ __device__ __forceinline__ void group_sync() {
 // is the share of every entry of it, four entries at a time, where wanted[i]. It comes back behind a
 // barrier of the group.
 template <typename T, typename IndexT, int kTPR, int kSlots>
-__device__ __forceinline__ void sum_shares(const Entries<T, IndexT, kTPR, kSlots>& entries, const int padded,
+__device__ __forceinline__ void sum_shares(const Entries<T, IndexT, kTPR, kSlots>& entries,
+                                           const typename IO<T>::Acc inv_t, const int padded,
                                            const bool (&wanted)[kSlots], int* classes,
                                            typename IO<T>::Acc* shares,
                                            typename IO<T>::Acc (*slots)[kTPR / kWaveSize],
@@ -553,13 +557,13 @@ __device__ __forceinline__ void sum_shares(const Entries<T, IndexT, kTPR, kSlots
                                            typename IO<T>::Acc (&share)[kSlots]) {
   using A = typename IO<T>::Acc;
   const int lane = static_cast<int>(threadIdx.x) % kTPR;
-  const ExpSum<A> t = entries.sum(slots);
+  const ExpSum<A> t = entries.sum(inv_t, slots);
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
     const int k = i * kTPR + lane;
     if (k < padded) {
       classes[k] = entries.cls[i];
-      shares[k] = entries.cls[i] >= 0 ? acc_exp(entries.z[i] - t.m) / t.s : A(0);
+      shares[k] = entries.cls[i] >= 0 ? acc_exp(entries.offset(i, t.m, inv_t)) / t.s : A(0);
     }
     // its logit has arrived before another thread may write over it
     asm volatile("" : "+v"(kept[i]));
@@ -612,7 +616,7 @@ __device__ __forceinline__ void far_row(const T* in, T* out, const int64_t C, co
     here[i] = entries.cls[i] >= 0;
     kept[i] = here[i] ? IO<T>::load1(in + entries.cls[i]) : A(0);
   }
-  sum_shares<T, IndexT, kTPR, kSlots>(entries, padded, here, classes, shares, slots, kept, share);
+  sum_shares<T, IndexT, kTPR, kSlots>(entries, inv_t, padded, here, classes, shares, slots, kept, share);
   const ExpSum<A> own = far_sum<T, kTPR>(in, C, inv_t, slots + 2);
   const A inv_s = A(1) / own.s;
 #pragma unroll 1
@@ -683,7 +687,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
     if (fabs(lse) > A(kFar / 2)) {
       if (!first) continue;
       Entries<T, IndexT, kTPR, kSlots> entries;
-      entries.load(row, C, K, inv_t, index, teacher);
+      entries.load(row, C, K, index, teacher);
       const A divisor = stats[N];
       const A w = dl[per_row ? row : 0] * temperature / (divisor > A(0.5) ? divisor : A(0.5));
       far_row<T, IndexT, kTPR, kSlots>(in, out, C, padded, entries, inv_t, w, classes, shares, slots);
@@ -703,7 +707,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
     if (first && lane < cut.tail) tail = IO<T>::load1(in + tail_at);
     // the teacher's shares
     Entries<T, IndexT, kTPR, kSlots> entries;
-    entries.load(row, C, K, inv_t, index, teacher);
+    entries.load(row, C, K, index, teacher);
     const A divisor = stats[N];
     const A w = dl[per_row ? row : 0] * temperature / (divisor > A(0.5) ? divisor : A(0.5));
     const A base = Math::from_log(lse);
@@ -718,7 +722,7 @@ __global__ __launch_bounds__(kSegmentThreads) void distill_backward_segments(
       kept[i] = here[i] ? IO<T>::load1(in + cls) : A(0);
     }
     A share[kSlots];
-    sum_shares<T, IndexT, kTPR, kSlots>(entries, padded, here, classes, shares, slots, kept, share);
+    sum_shares<T, IndexT, kTPR, kSlots>(entries, inv_t, padded, here, classes, shares, slots, kept, share);
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) kept[i] = w * (Math::term(kept[i], scale, base) - share[i]);
     if (first && lane < cut.head) IO<T>::store1(out + lane, w * Math::term(head, scale, base));

@@ -1,0 +1,50 @@
+"""The operators of language models at the edges of their ranges: logits and probabilities at which roundings decide,
+tensors and extents beyond 31 bits, gradients that reach an operator by one of its outputs alone."""
+
+import numpy as np
+import pytest
+import torch
+
+from tests import language_ops as L
+from tests.test_gpu_language_ops import DTYPES, _distill_case, _run_distill
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(7, 130, 3), (7, 4200, 300), (7, 9001, 5), (7, 70001, 9)])
+@pytest.mark.parametrize("temperature", [0.5, 0.75, 1.5])
+def test_distillation_of_teachers_far_from_zero(dtype, shape, temperature):
+    """The teacher's shares depend on differences of its logits alone, so the plain form is that of the rows less
+    their largest listed logit (exact in 64 bits), with its bounds; entries that are 800 and more below it have
+    a share of exactly 0 in every type and are not listed there."""
+    N, C, k = shape
+    x, index, teacher = _distill_case(N, C, k, dtype, torch.int32, 21, 2.0)
+    g = torch.Generator().manual_seed(4)
+    index.copy_(torch.randint(0, C, (N, k), generator=g))
+    teacher.copy_(torch.randn((N, k), generator=g, dtype=torch.float64) * 2)
+    low = torch.finfo(teacher.dtype).min
+    teacher[0] += 30000
+    teacher[1] -= 30000
+    teacher[2] = low                  # nothing but the type's lowest value: equal shares
+    teacher[3] = low                  # one entry is left
+    teacher[3, k - 1] = 1.0
+    teacher[4] = -low / 2             # far above zero
+    teacher[4, 0] = low
+    teacher[5, 0] = -float("inf")     # not listed
+    teacher[5, 1:] += 1e6
+    dl = torch.rand(N, generator=g).to(teacher.dtype).cuda()
+    stats, loss, dx = _run_distill(x, index, teacher, temperature, "NONE", dl)
+    t = L.f64(teacher)
+    with np.errstate(over="ignore"):
+        shifted = t - t.max(1, keepdims=True)
+        near = shifted / temperature > -800
+    plain = (L.f64(x), np.where(near, index.cpu().numpy().astype(np.int64), -1), np.where(near, shifted, 0.0))
+    ws_, rows, _ = L.distill_forward(temperature, "NONE", *plain)
+    b_lse, b_rows = L.distill_bounds(dtype, temperature, *plain)
+    L.assert_close(L.f64(loss), rows, b_rows, "loss")
+    L.assert_close(L.f64(stats)[:N], ws_[:N], b_lse, "lse")
+    got_stats = L.f64(stats)
+    want, s, sh = L.distill_backward(temperature, "NONE", *plain, got_stats, L.f64(dl))
+    L.assert_close(L.f64(dx), want, L.distill_grad_bound(dtype, temperature, plain[0], plain[2], plain[1], got_stats, want,
+                                                         s, sh), "dx")
