@@ -7,14 +7,14 @@ namespace dragon {
 
 namespace {
 
-// 0 keeps a loss per row, -1 divides by the rows that count.
-float DistillationNormalizer(const string& reduction, int64_t rows, int64_t dim0) {
+// 0 keeps a loss per row, -1 divides by the rows that count. Logits without leading axes are one row.
+float DistillationNormalizer(const string& reduction, int64_t rows, const Tensor& X) {
   if (reduction == "NONE") return 0.f;
   if (reduction == "VALID") return -1.f;
   if (reduction == "SUM") return 1.f;
   // of no rows, the sum is 0 whatever divides it
   if (reduction == "MEAN") return static_cast<float>(rows > 0 ? rows : 1);
-  if (reduction == "BATCH_MEAN") return static_cast<float>(dim0 > 0 ? dim0 : 1);
+  if (reduction == "BATCH_MEAN") return X.ndim() > 1 && X.dim(0) > 0 ? static_cast<float>(X.dim(0)) : 1.f;
   LOG(FATAL) << "Unknown reduction: " << reduction;
   return 0.f;
 }
@@ -60,7 +60,7 @@ void TopKDistillationLossOp<Context>::DoRunWithIndex() {
   if (reduction_ != "NONE") out_dims.clear();
   kernels::TopKDistillationLossForward(
       static_cast<int>(rows), static_cast<int>(X.dim(-1)), static_cast<int>(I.dim(-1)), temperature_,
-      DistillationNormalizer(reduction_, rows, X.dim(0)), X.template data<T, Context>(ctx()),
+      DistillationNormalizer(reduction_, rows, X), X.template data<T, Context>(ctx()),
       I.template data<IndexT, Context>(ctx()), Input(2).template data<AccT, Context>(ctx()),
       Output("X_stats")->Reshape({rows + 1})->template mutable_data<AccT, Context>(ctx()),
       Output(0)->Reshape(out_dims)->template mutable_data<AccT, Context>(ctx()), ctx());
@@ -91,7 +91,7 @@ void TopKDistillationLossGradientOp<Context>::DoRunWithIndex() {
   CHECK_EQ(Input("X_stats").count(), rows + 1) << "\nThe forward operator saw other logits.";
   kernels::TopKDistillationLossBackward(
       static_cast<int>(rows), static_cast<int>(X.dim(-1)), static_cast<int>(I.dim(-1)), temperature_,
-      DistillationNormalizer(reduction_, rows, X.dim(0)), X.template data<T, Context>(ctx()),
+      DistillationNormalizer(reduction_, rows, X), X.template data<T, Context>(ctx()),
       I.template data<IndexT, Context>(ctx()), Input(2).template data<AccT, Context>(ctx()),
       Input("X_stats").template data<AccT, Context>(ctx()), dL.template data<AccT, Context>(ctx()),
       Output(0)->ReshapeLike(X)->template mutable_data<T, Context>(ctx()), ctx());

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import language_ops as L
-from tests.test_gpu_language_ops import DTYPES, _distill_case, _run_distill
+from tests.test_gpu_language_ops import DTYPES, _distill_case, _run_distill, ws  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,20 @@ def test_distillation_of_teachers_far_from_zero(dtype, shape, temperature):
     want, s, sh = L.distill_backward(temperature, "NONE", *plain, got_stats, L.f64(dl))
     L.assert_close(L.f64(dx), want, L.distill_grad_bound(dtype, temperature, plain[0], plain[2], plain[1], got_stats, want,
                                                          s, sh), "dx")
+
+
+@pytest.mark.parametrize("reduction", ["batch_mean", "mean", "valid"])
+def test_operator_topk_distillation_loss_of_one_row_of_logits(ws, reduction):
+    """Logits [C] without leading axes are one row."""
+    from dragon_amd import runtime as rt
+    rng = np.random.default_rng(9)
+    x, t, i = rng.standard_normal(50), rng.standard_normal(4), rng.integers(0, 50, 4)
+    for n, a in (("x", x), ("i", i), ("t", t), ("dl", np.array(0.5))):
+        ws.feed(n, a)
+    tape = rt.Tape(ws)
+    loss = rt.topk_distillation_loss(tape, ["x", "i", "t"], temperature=2.0, reduction=reduction)
+    (dx,) = tape.gradient(loss, ["x"], output_gradient="dl")
+    stats, _, want = L.distill_forward(2.0, "MEAN", x[None], i[None], t[None])
+    grad, _, _ = L.distill_backward(2.0, "MEAN", x[None], i[None], t[None], stats, np.array([0.5]))
+    assert ws.info(loss)[1] == () and np.allclose(ws.fetch(loss), want, rtol=1e-12)
+    assert np.allclose(ws.fetch(dx), grad[0], rtol=1e-12, atol=1e-15)
