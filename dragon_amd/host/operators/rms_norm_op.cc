@@ -1,11 +1,24 @@
 #include "operators/rms_norm_op.h"
 
-#include <climits>
+#include <algorithm>
 
 #include "core/gradient.h"
 #include "kernels/op_kernels.h"
 
 namespace dragon {
+
+namespace {
+
+// math::Copy counts in int; tensors of these operators may hold more elements.
+template <typename T, class Context>
+void CopyElements(const int64_t n, const T* x, T* y, Context* ctx) {
+  constexpr int64_t kMost = int64_t(1) << 30;
+  for (int64_t at = 0; at < n; at += kMost) {
+    math::Copy(static_cast<int>(std::min(kMost, n - at)), x + at, y + at, ctx);
+  }
+}
+
+} // namespace
 
 template <class Context>
 template <typename T>
@@ -52,9 +65,8 @@ void RMSNormGradientOp<Context>::DoRunWithType() {
                        W.template data<AccT, Context>(ctx()), Input(2).template data<T, Context>(ctx()), dh,
                        Output(1)->ReshapeLike(W)->template mutable_data<AccT, Context>(ctx()), dx, ctx());
   if (OutputSize() > 2) {  // X and the residual are summed: one gradient for both, in a tensor each
-    CHECK_LE(H.count(), static_cast<int64_t>(INT_MAX)) << "\nToo many elements for a copied gradient.";
-    math::Copy(static_cast<int>(H.count()), static_cast<const T*>(dx),
-               Output(2)->ReshapeLike(H)->template mutable_data<T, Context>(ctx()), ctx());
+    CopyElements(H.count(), static_cast<const T*>(dx),
+                 Output(2)->ReshapeLike(H)->template mutable_data<T, Context>(ctx()), ctx());
   }
 }
 

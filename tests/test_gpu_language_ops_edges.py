@@ -65,3 +65,42 @@ def test_operator_topk_distillation_loss_of_one_row_of_logits(ws, reduction):
     grad, _, _ = L.distill_backward(2.0, "MEAN", x[None], i[None], t[None], stats, np.array([0.5]))
     assert ws.info(loss)[1] == () and np.allclose(ws.fetch(loss), want, rtol=1e-12)
     assert np.allclose(ws.fetch(dx), grad[0], rtol=1e-12, atol=1e-15)
+
+
+def test_operator_rms_norm_gradient_of_more_than_2_31_elements(ws):
+    """With a residual: its gradient is in a tensor of its own, equal to that of X to the last row."""
+    from dragon_amd import runtime as rt
+    C = 4096
+    N = (1 << 31) // C + 5
+    rng = np.random.default_rng(3)
+    bits = lambda shape, seed: torch.randn(shape, generator=torch.Generator().manual_seed(seed)).bfloat16().view(torch.uint16).numpy()
+    at = np.array([0, 1, N - 6, N - 5, N - 2, N - 1])
+    parts = {}
+    for i, n in enumerate(("x", "r", "dy")):
+        a = np.zeros((N, C), np.uint16)
+        parts[n] = bits((len(at), C), i)
+        a[at] = parts[n]
+        ws.feed(n, a, dtype="bfloat16", device=("hip", 0))
+        del a
+    w = rng.uniform(0.5, 1.5, C).astype(np.float32)
+    ws.feed("w", w)
+    tape = rt.Tape(ws)
+    y, h = rt.rms_norm(tape, ["x", "w", "r"])
+    dx, dw, dr = tape.gradient(y, ["x", "w", "r"], output_gradient="dy")
+    f = {n: torch.from_numpy(v).view(torch.bfloat16).double().numpy() for n, v in parts.items()}
+    got = ws.fetch(dr)
+    assert got.shape == (N, C)
+    rest = np.ones(N, bool)
+    rest[at] = False
+    assert not got[:2000][rest[:2000]].any() and not got[-2000:][rest[-2000:]].any()
+    tail = got[at].copy()
+    del got
+    assert np.array_equal(ws.fetch(dx)[at], tail)
+    hs = torch.from_numpy(ws.fetch(h)[at]).view(torch.bfloat16).double().numpy()
+    _, rs, _ = L.rms_norm(f["x"] + f["r"], None, w.astype(np.float64), float(np.float32(1e-5)))
+    args = (hs, rs, w.astype(np.float64), f["dy"], None)
+    want, want_g = L.rms_norm_grad(*args)
+    bx, _ = L.rms_norm_grad_bounds("bfloat16", *args, want)
+    # rsig is the kernel's own, off by (DEPTH / 2 + 3) roundings; dx holds its third power at most
+    L.assert_close(torch.from_numpy(tail).view(torch.bfloat16).double().numpy(), want,
+                   bx + 3 * (L.DEPTH / 2 + 3) * 2.0 ** -24 * (np.abs(want) + np.abs(f["dy"] * w) * rs[:, None]), "dx")
