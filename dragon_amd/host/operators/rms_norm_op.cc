@@ -72,6 +72,22 @@ void RMSNormGradientOp<Context>::DoRunWithType() {
 
 template <class Context>
 template <typename T>
+void RMSNormSumGradientOp<Context>::DoRunWithType() {
+  using AccT = typename math::Traits<T>::accumulator_type;
+  Tensor& dH = Input(0);
+  Tensor& W = Input(1);
+  GET_OP_AXIS_ARG(axis, dH.ndim(), -1);
+  const int64_t width = dH.count(axis);
+  INITIALIZE_TENSOR_VIA_SPEC(W, vec64_t({width}), AccT);
+  const T* dh = dH.template data<T, Context>(ctx());
+  CopyElements(dH.count(), dh, Output(0)->ReshapeLike(dH)->template mutable_data<T, Context>(ctx()), ctx());
+  math::Set(static_cast<int>(width), AccT(0),
+            Output(1)->ReshapeLike(W)->template mutable_data<AccT, Context>(ctx()), ctx());
+  CopyElements(dH.count(), dh, Output(2)->ReshapeLike(dH)->template mutable_data<T, Context>(ctx()), ctx());
+}
+
+template <class Context>
+template <typename T>
 void RMSNormQuantOp<Context>::DoRunWithType() {
   Tensor& X = Input(0);
   Tensor& W = Input(1);
@@ -99,10 +115,12 @@ void RMSNormQuantOp<Context>::DoRunWithType() {
 
 DEPLOY_HIP_OPERATOR(RMSNorm);
 DEPLOY_HIP_OPERATOR(RMSNormGradient);
+DEPLOY_HIP_OPERATOR(RMSNormSumGradient);
 DEPLOY_HIP_OPERATOR(RMSNormQuant);
 
 OPERATOR_SCHEMA(RMSNorm).NumInputs(2, 3).NumOutputs(1, 2);          // X, W[, R] -> Y[, H]
 OPERATOR_SCHEMA(RMSNormGradient).NumInputs(3, 4).NumOutputs(2, 3);  // H, W, dY[, dH] -> dX, dW[, dR]
+OPERATOR_SCHEMA(RMSNormSumGradient).NumInputs(2).NumOutputs(3);     // dH, W -> dX, dW, dR
 OPERATOR_SCHEMA(RMSNormQuant).NumInputs(2, 3).NumOutputs(2, 3);     // X, W[, R] -> Q, S[, H]
 
 namespace {
@@ -115,10 +133,19 @@ class RMSNormGradientMaker final : public GradientMakerBase {
       AddGradientDef("RMSNormGradient", {I(0), I(1), GO(0)}, {GI(0), GI(1)});
       return;
     }
+    const bool from_y = Arrives(0), from_h = Arrives(1);
+    CHECK(from_y || from_h) << "\nNo gradient arrives at Operator(" << def().type << ").";
+    if (!from_y) {  // what arrives at the sum passes on as it is
+      AddGradientDef("RMSNormSumGradient", {GO(1), I(1)}, {GI(0), GI(1), GI(2)});
+      return;
+    }
     vector<string> inputs = {O(1), I(1), GO(0)};
-    if (!GO(1).empty() && GO(1) != "NULL") inputs.push_back(GO(1));
+    if (from_h) inputs.push_back(GO(1));
     AddGradientDef("RMSNormGradient", inputs, {GI(0), GI(1), GI(2)});
   }
+
+ private:
+  bool Arrives(int i) const { return !GO(i).empty() && GO(i) != "NULL"; }
 };
 
 } // namespace

@@ -4,6 +4,7 @@
 //                    X, W, R       -> Y, H         H = X + R, Y the norm of H
 //   RMSNormGradient  X, W, dY      -> dX, dW
 //                    H, W, dY[, dH] -> dX, dW, dR  dH: what arrives through H; dR equals dX
+//   RMSNormSumGradient  dH, W     -> dX, dW, dR    where nothing arrives through Y: dX = dR = dH, dW = 0
 //   RMSNormQuant     X, W[, R]     -> Q, S[, H]    Q e4m3 codes (uint8), S float32 scales: one per
 //                                                  "group_size" columns, or per row for 0
 //
@@ -50,6 +51,7 @@ struct QuantDispatch {
 
 DECLARE_RMS_NORM_OP(RMSNorm, FloatingDispatch)
 DECLARE_RMS_NORM_OP(RMSNormGradient, FloatingDispatch)
+DECLARE_RMS_NORM_OP(RMSNormSumGradient, FloatingDispatch)
 DECLARE_RMS_NORM_OP(RMSNormQuant, QuantDispatch)
 #undef DECLARE_RMS_NORM_OP
 

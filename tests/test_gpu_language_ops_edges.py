@@ -104,3 +104,59 @@ def test_operator_rms_norm_gradient_of_more_than_2_31_elements(ws):
     # rsig is the kernel's own, off by (DEPTH / 2 + 3) roundings; dx holds its third power at most
     L.assert_close(torch.from_numpy(tail).view(torch.bfloat16).double().numpy(), want,
                    bx + 3 * (L.DEPTH / 2 + 3) * 2.0 ** -24 * (np.abs(want) + np.abs(f["dy"] * w) * rs[:, None]), "dx")
+
+
+def test_operator_rms_norm_gradients_through_a_chain(ws):
+    """Two residual norms with Softmax between them, the stream through both: Tape.gradient from the last norm, from
+    the last sum and from the first sum against torch's derivatives in float64."""
+    from dragon_amd import runtime as rt
+    rng = np.random.default_rng(11)
+    a = {n: rng.standard_normal((2, 5, 24)) for n in ("x", "r")}
+    a.update({n: rng.uniform(0.5, 1.5, 24) for n in ("w1", "w2")})
+    d = rng.standard_normal((2, 5, 24))
+    for n in a:
+        ws.feed(n, a[n])
+    ws.feed("d", d)
+    t = {n: torch.from_numpy(v).requires_grad_() for n, v in a.items()}
+    eps = float(np.float32(1e-5))
+    norm = lambda s, w: s / torch.sqrt(s.square().mean(-1, keepdim=True) + eps) * w
+    h1 = t["x"] + t["r"]
+    m = torch.softmax(norm(h1, t["w1"]), -1)
+    h2 = m + h1
+    y2 = norm(h2, t["w2"])
+
+    tape = rt.Tape(ws)
+    o1, s1 = rt.rms_norm(tape, ["x", "w1", "r"])
+    mid = rt.softmax(tape, [o1])
+    o2, s2 = rt.rms_norm(tape, [mid, "w2", s1])
+    sources = ["x", "w1", "r", "w2"]
+    for target, value, reached in ((o2, y2, sources), (s2, h2, sources), (s1, h1, ["x", "w1", "r"])):
+        want = torch.autograd.grad((value * torch.from_numpy(d)).sum(), [t[n] for n in reached], retain_graph=True,
+                                   allow_unused=True)
+        got = tape.gradient(target, reached, output_gradient="d")
+        for n, g, w in zip(reached, got, want):
+            w = np.zeros_like(a[n]) if w is None else w.numpy()
+            # chains of a hundred roundings in 64 bits on values of order 1 to 10
+            assert np.abs(ws.fetch(g) - w).max() < 1e-13, (target, n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_operator_rms_norm_gradient_through_the_sum_alone(ws, dtype):
+    """dX and dR are dH, bit for bit, and dW is zero."""
+    from dragon_amd import runtime as rt
+    raw = {"bfloat16": "bfloat16", "float16": "float16"}.get(dtype)
+    acc = np.float64 if dtype == "float64" else np.float32
+    def feed(name, shape, seed):
+        v = torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(getattr(torch, dtype))
+        ws.feed(name, v.view(torch.uint16).numpy() if raw else v.numpy(), dtype=raw)
+    for shape in ((3, 7, 50), (0, 50)):
+        for i, n in enumerate(("x", "r", "dh")):
+            feed(n, shape, i)
+        ws.feed("w", np.ones(50, acc))
+        tape = rt.Tape(ws)
+        y, h = rt.rms_norm(tape, ["x", "w", "r"])
+        dx, dw, dr = tape.gradient(h, ["x", "w", "r"], output_gradient="dh")
+        want = ws.fetch("dh", raw=True)
+        for g in (dx, dr):
+            assert ws.info(g) == (dtype, shape) and np.array_equal(ws.fetch(g, raw=True), want)
+        assert ws.info(dw)[1] == (50,) and not ws.fetch(dw).any()

@@ -150,6 +150,34 @@ def test_plans_by_size():
     assert "draft_verify_runs" in plan("draft_verify", (512, 4, 1 << 20), "float32")
 
 
+# ---------------------------------------------------------------- the operators of the host layer
+
+@pytest.fixture()
+def ws():
+    from dragon_amd import runtime
+    w = runtime.Workspace("language_ops_host_test")
+    yield w
+    w.close()
+
+
+def test_gradient_definitions_of_rms_norm_by_what_arrives(ws):
+    """A definition names no tensor that does not exist: neither "NULL" nor "" is an input of its own."""
+    from dragon_amd import runtime as rt
+    forward = rt.make_def("RMSNorm", ["x", "w", "r"], ["y", "h"], name="n", axis=-1, epsilon=1e-3)
+    grads = ["x_grad", "w_grad", "r_grad"]
+    for none in ("NULL", ""):
+        for arriving, op, inputs in ((["dy", "dh"], "RMSNormGradient", ["h", "w", "dy", "dh"]),
+                                     (["dy", none], "RMSNormGradient", ["h", "w", "dy"]),
+                                     ([none, "dh"], "RMSNormSumGradient", ["dh", "w"])):
+            (text,), names = ws.gradient_defs(forward, arriving)
+            assert names == grads and 'type: "%s"' % op in text
+            assert [p.split('"')[1] for p in text.split("input: ")[1:]] == inputs
+            assert [p.split('"')[1] for p in text.split("output: ")[1:]] == grads
+        with pytest.raises(rt.DragonError, match="No gradient"):
+            ws.gradient_defs(forward, [none, none])
+    assert "RMSNormSumGradient" in rt.registered_operators()
+
+
 # ---------------------------------------------------------------- the plain forms themselves
 
 def test_plain_distillation_is_the_divergence_of_torch():
