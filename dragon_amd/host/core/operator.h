@@ -4,6 +4,8 @@
 // normalisation and softmax operators use.
 #pragma once
 
+#include <climits>
+
 #include "core/common.h"
 #include "core/context.h"
 #include "core/operator_def.h"
@@ -120,6 +122,12 @@ class Operator : public OperatorBase {
         << "\nExcepted Tensor(" << (tensor).name() << ")'s dimensions are "             \
         << DimsToString(expected_shape) << ", got " << DimsToString((tensor).dims()) << "."; \
   } while (0)
+
+// An extent that a kernel counts in int, refused where it would be cut to another one.
+inline int KernelExtent(const char* what, int64_t n) {
+  CHECK_LE(n, int64_t(INT_MAX)) << "\nToo large an extent: " << what << ".";
+  return static_cast<int>(n);
+}
 
 // Calls op->DoRunWithType<T>() for the floating type of `tensor`
 // (DispatchHelper<dtypes::Floating>, dragon/core/operator.h:256-296).

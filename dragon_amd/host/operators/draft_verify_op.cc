@@ -21,7 +21,8 @@ template <typename T, typename IndexT>
 void DraftVerifyOp<Context>::DoRunWithIndex() {
   Tensor& P = Input(0);
   CHECK_EQ(P.ndim(), 3) << "\nExcepted probabilities of shape (B, K + 1, C).";
-  const int64_t B = P.dim(0), K = P.dim(1) - 1, C = P.dim(2);
+  const int64_t B = KernelExtent("sequences", P.dim(0)), K = KernelExtent("drafted tokens", P.dim(1) - 1);
+  const int64_t C = KernelExtent("classes", P.dim(2));
   CHECK_GE(K, 0) << "\nExcepted probabilities at one position at least.";
   INITIALIZE_TENSOR_VIA_SPEC(Input(1), vec64_t({B, K}), IndexT);
   INITIALIZE_TENSOR_VIA_SPEC(Input(2), vec64_t({B}), IndexT);

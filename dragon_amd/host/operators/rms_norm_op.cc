@@ -27,7 +27,7 @@ void RMSNormOp<Context>::DoRunWithType() {
   Tensor& X = Input(0);
   Tensor& W = Input(1);
   GET_OP_AXIS_ARG(axis, X.ndim(), -1);
-  const int64_t rows = X.count(0, axis), width = X.count(axis);
+  const int rows = KernelExtent("rows", X.count(0, axis)), width = KernelExtent("columns", X.count(axis));
   INITIALIZE_TENSOR_VIA_SPEC(W, vec64_t({width}), AccT);
   CHECK_EQ(OutputSize(), InputSize() - 1) << "\nA residual's sum is the second output.";
   const T* residual = nullptr;
@@ -37,7 +37,7 @@ void RMSNormOp<Context>::DoRunWithType() {
     residual = Input(2).template data<T, Context>(ctx());
     h = Output(1)->ReshapeLike(X)->template mutable_data<T, Context>(ctx());
   }
-  kernels::RMSNorm(static_cast<int>(rows), static_cast<int>(width), static_cast<float>(epsilon_),
+  kernels::RMSNorm(rows, width, static_cast<float>(epsilon_),
                    X.template data<T, Context>(ctx()), residual, W.template data<AccT, Context>(ctx()), h,
                    Output("X_rsig")->Reshape({rows})->template mutable_data<AccT, Context>(ctx()),
                    Output(0)->ReshapeLike(X)->template mutable_data<T, Context>(ctx()), ctx());
@@ -50,7 +50,7 @@ void RMSNormGradientOp<Context>::DoRunWithType() {
   Tensor& H = Input(0);
   Tensor& W = Input(1);
   GET_OP_AXIS_ARG(axis, H.ndim(), -1);
-  const int64_t rows = H.count(0, axis), width = H.count(axis);
+  const int rows = KernelExtent("rows", H.count(0, axis)), width = KernelExtent("columns", H.count(axis));
   INITIALIZE_TENSOR_VIA_SPEC(W, vec64_t({width}), AccT);
   INITIALIZE_TENSOR_VIA_SPEC(Input(2), H.dims(), T);
   const T* dh = nullptr;
@@ -59,7 +59,7 @@ void RMSNormGradientOp<Context>::DoRunWithType() {
     dh = Input(3).template data<T, Context>(ctx());
   }
   T* dx = Output(0)->ReshapeLike(H)->template mutable_data<T, Context>(ctx());
-  kernels::RMSNormGrad(static_cast<int>(rows), static_cast<int>(width),
+  kernels::RMSNormGrad(rows, width,
                        H.template data<T, Context>(ctx()),
                        Input("X_rsig").template data<AccT, Context>(ctx()),
                        W.template data<AccT, Context>(ctx()), Input(2).template data<T, Context>(ctx()), dh,
@@ -77,11 +77,11 @@ void RMSNormSumGradientOp<Context>::DoRunWithType() {
   Tensor& dH = Input(0);
   Tensor& W = Input(1);
   GET_OP_AXIS_ARG(axis, dH.ndim(), -1);
-  const int64_t width = dH.count(axis);
+  const int width = KernelExtent("columns", dH.count(axis));
   INITIALIZE_TENSOR_VIA_SPEC(W, vec64_t({width}), AccT);
   const T* dh = dH.template data<T, Context>(ctx());
   CopyElements(dH.count(), dh, Output(0)->ReshapeLike(dH)->template mutable_data<T, Context>(ctx()), ctx());
-  math::Set(static_cast<int>(width), AccT(0),
+  math::Set(width, AccT(0),
             Output(1)->ReshapeLike(W)->template mutable_data<AccT, Context>(ctx()), ctx());
   CopyElements(dH.count(), dh, Output(2)->ReshapeLike(dH)->template mutable_data<T, Context>(ctx()), ctx());
 }
@@ -92,10 +92,11 @@ void RMSNormQuantOp<Context>::DoRunWithType() {
   Tensor& X = Input(0);
   Tensor& W = Input(1);
   GET_OP_AXIS_ARG(axis, X.ndim(), -1);
-  const int64_t rows = X.count(0, axis), width = X.count(axis);
+  const int rows = KernelExtent("rows", X.count(0, axis)), width = KernelExtent("columns", X.count(axis));
   INITIALIZE_TENSOR_VIA_SPEC(W, vec64_t({width}), float);
   CHECK_EQ(OutputSize(), InputSize()) << "\nA residual's sum is the third output.";
   CHECK_GE(group_size_, 0) << "\nExcepted a <group_size> of 0, 32, 64, 128 or 256.";
+  const int group_size = KernelExtent("group_size", group_size_);
   const T* residual = nullptr;
   T* h = nullptr;
   if (InputSize() > 2) {
@@ -104,9 +105,9 @@ void RMSNormQuantOp<Context>::DoRunWithType() {
     h = Output(2)->ReshapeLike(X)->template mutable_data<T, Context>(ctx());
   }
   vec64_t scale_dims(X.dims().begin(), X.dims().begin() + axis);
-  scale_dims.push_back(group_size_ > 0 ? (width + group_size_ - 1) / group_size_ : 1);
+  scale_dims.push_back(group_size > 0 ? (int64_t(width) + group_size - 1) / group_size : 1);
   kernels::RMSNormQuant(
-      static_cast<int>(rows), static_cast<int>(width), static_cast<int>(group_size_),
+      rows, width, group_size,
       static_cast<float>(epsilon_), X.template data<T, Context>(ctx()), residual,
       W.template data<float, Context>(ctx()), h, static_cast<float*>(nullptr),
       Output(0)->ReshapeLike(X)->template mutable_data<uint8_t, Context>(ctx()),

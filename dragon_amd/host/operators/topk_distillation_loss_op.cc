@@ -55,11 +55,12 @@ void TopKDistillationLossOp<Context>::DoRunWithIndex() {
   Tensor& X = Input(0);
   Tensor& I = Input(1);
   CheckShapes<AccT>(X, I, Input(2));
-  const int64_t rows = X.count(0, X.ndim() - 1);
+  const int64_t rows = KernelExtent("rows", X.count(0, X.ndim() - 1));
+  const int classes = KernelExtent("classes", X.dim(-1)), listed = KernelExtent("listed classes", I.dim(-1));
   vec64_t out_dims(X.dims().begin(), X.dims().end() - 1);
   if (reduction_ != "NONE") out_dims.clear();
   kernels::TopKDistillationLossForward(
-      static_cast<int>(rows), static_cast<int>(X.dim(-1)), static_cast<int>(I.dim(-1)), temperature_,
+      static_cast<int>(rows), classes, listed, temperature_,
       DistillationNormalizer(reduction_, rows, X), X.template data<T, Context>(ctx()),
       I.template data<IndexT, Context>(ctx()), Input(2).template data<AccT, Context>(ctx()),
       Output("X_stats")->Reshape({rows + 1})->template mutable_data<AccT, Context>(ctx()),
@@ -86,11 +87,12 @@ void TopKDistillationLossGradientOp<Context>::DoRunWithIndex() {
   Tensor& I = Input(1);
   Tensor& dL = Input(3);
   CheckShapes<AccT>(X, I, Input(2));
-  const int64_t rows = X.count(0, X.ndim() - 1);
+  const int64_t rows = KernelExtent("rows", X.count(0, X.ndim() - 1));
+  const int classes = KernelExtent("classes", X.dim(-1)), listed = KernelExtent("listed classes", I.dim(-1));
   CHECK_EQ(dL.count(), reduction_ == "NONE" ? rows : 1) << "\nNumel of L and dL must be matched.";
   CHECK_EQ(Input("X_stats").count(), rows + 1) << "\nThe forward operator saw other logits.";
   kernels::TopKDistillationLossBackward(
-      static_cast<int>(rows), static_cast<int>(X.dim(-1)), static_cast<int>(I.dim(-1)), temperature_,
+      static_cast<int>(rows), classes, listed, temperature_,
       DistillationNormalizer(reduction_, rows, X), X.template data<T, Context>(ctx()),
       I.template data<IndexT, Context>(ctx()), Input(2).template data<AccT, Context>(ctx()),
       Input("X_stats").template data<AccT, Context>(ctx()), dL.template data<AccT, Context>(ctx()),

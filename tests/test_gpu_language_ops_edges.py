@@ -160,3 +160,54 @@ def test_operator_rms_norm_gradient_through_the_sum_alone(ws, dtype):
         for g in (dx, dr):
             assert ws.info(g) == (dtype, shape) and np.array_equal(ws.fetch(g, raw=True), want)
         assert ws.info(dw)[1] == (50,) and not ws.fetch(dw).any()
+
+
+def test_operators_refuse_extents_that_their_kernels_do_not_count(ws):
+    from dragon_amd import runtime as rt
+    huge = (1 << 32) + 3  # 3 rows, were it cut to 32 bits
+    ws.feed("x", np.zeros((huge, 1), np.float16))
+    ws.feed("w", np.zeros(1, np.float32))
+    with pytest.raises(rt.DragonError, match="2147483647"):
+        ws.run_operator(rt.make_def("RMSNorm", ["x", "w"], ["y"]))
+
+
+@pytest.mark.parametrize("op,inputs,outputs", [("RMSNorm", "xw", 1), ("RMSNormQuant", "xw", 2), ("RMSNormGradient", "xwx", 2),
+                                               ("TopKDistillationLoss", "xit", 1), ("TopKDistillationLossGradient", "xitw", 1),
+                                               ("DraftVerify", "pintw", 2)])
+def test_operators_name_the_extents_they_refuse(ws, op, inputs, outputs):
+    """Without elements, so without memory."""
+    from dragon_amd import runtime as rt
+    huge = (1 << 32) + 3
+    for n, shape, dtype in (("x", (huge, 0), np.float32), ("w", (0,), np.float32), ("i", (huge, 0), np.int64), ("n", (0,), np.int64),
+                            ("t", (huge, 0), np.float32), ("p", (huge, 1, 0), np.float32)):
+        ws.feed(n, np.zeros(shape, dtype))
+    with pytest.raises(rt.DragonError, match="2147483647"):
+        ws.run_operator(rt.make_def(op, list(inputs), ["o%d" % i for i in range(outputs)]))
+    if op == "RMSNormQuant":
+        ws.feed("x", np.zeros((2, 64), np.float32))
+        ws.feed("w", np.zeros(64, np.float32))
+        with pytest.raises(rt.DragonError, match="2147483647"):  # groups of 32, were it cut
+            ws.run_operator(rt.make_def(op, ["x", "w"], ["q", "s"], group_size=(1 << 32) + 32))
+
+
+def test_operators_of_empty_batches_and_without_drafts(ws):
+    from dragon_amd import runtime as rt
+    f = lambda *s: np.zeros(s, np.float32)
+    for n, a in (("x", f(0, 8)), ("w", f(8)), ("i", np.zeros((0, 2), np.int64)), ("t", f(0, 2)), ("dy", f(0, 8)), ("one", np.ones((), np.float32))):
+        ws.feed(n, a)
+    tape = rt.Tape(ws)
+    y, h = rt.rms_norm(tape, ["x", "w", "x"])
+    assert ws.info(y)[1] == (0, 8)
+    y = rt.rms_norm(tape, ["x", "w"])
+    dx, dw = tape.gradient(y, ["x", "w"], output_gradient="dy")
+    assert ws.info(dx)[1] == (0, 8) and not ws.fetch(dw).any()
+    loss = rt.topk_distillation_loss(tape, ["x", "i", "t"])
+    assert float(ws.fetch(loss)) == 0
+    (dx,) = tape.gradient(loss, ["x"], output_gradient="one")
+    assert ws.info(dx)[1] == (0, 8)
+    p = np.random.default_rng(1).random((3, 1, 9)).astype(np.float32)
+    for n, a in (("p", p), ("d", np.zeros((3, 0), np.int64)), ("n", np.zeros(3, np.int64)), ("ua", f(3, 0)), ("us", f(3)), ("q", f(3, 0, 9))):
+        ws.feed(n, a)
+    for inputs in (["p", "d", "n", "ua", "us"], ["p", "d", "n", "ua", "us", "q"]):
+        tokens, accepted = rt.draft_verify(tape, inputs)
+        assert not ws.fetch(accepted).any() and not ws.fetch(tokens).any()  # u = 0: the first class
