@@ -53,6 +53,7 @@ void RMSNormGradientOp<Context>::DoRunWithType() {
   const int rows = KernelExtent("rows", H.count(0, axis)), width = KernelExtent("columns", H.count(axis));
   INITIALIZE_TENSOR_VIA_SPEC(W, vec64_t({width}), AccT);
   INITIALIZE_TENSOR_VIA_SPEC(Input(2), H.dims(), T);
+  CHECK_EQ(Input("X_rsig").count(), rows) << "\nThe forward operator saw other rows.";
   const T* dh = nullptr;
   if (InputSize() > 3) {
     INITIALIZE_TENSOR_VIA_SPEC(Input(3), H.dims(), T);

@@ -211,3 +211,18 @@ def test_operators_of_empty_batches_and_without_drafts(ws):
     for inputs in (["p", "d", "n", "ua", "us"], ["p", "d", "n", "ua", "us", "q"]):
         tokens, accepted = rt.draft_verify(tape, inputs)
         assert not ws.fetch(accepted).any() and not ws.fetch(tokens).any()  # u = 0: the first class
+
+
+def test_operator_rms_norm_gradient_of_other_rows_than_the_forward_saw(ws):
+    """The kept reciprocal roots are as many as the rows: more rows would read behind them."""
+    from dragon_amd import runtime as rt
+    f = lambda *s: np.ones(s, np.float32)
+    for n, a in (("x", f(2, 8)), ("w", f(8)), ("more", f(2000, 8)), ("less", f(1, 8))):
+        ws.feed(n, a)
+    tape = rt.Tape(ws)
+    rt.rms_norm(tape, ["x", "w"])
+    (text,), _ = ws.gradient_defs(tape.records[-1][0], ["x"])
+    ws.run_operator(text)
+    for other in ("more", "less"):
+        with pytest.raises(rt.DragonError, match="other rows"):
+            ws.run_operator(text.replace('input: "x"', 'input: "%s"' % other))
