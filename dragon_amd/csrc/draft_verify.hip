@@ -263,7 +263,8 @@ __device__ __forceinline__ int64_t pick_class(SampleRow<T> row, const int64_t C,
     });
     __syncthreads();
   }
-  const double level = u > 0.f ? static_cast<double>(u) * total : 0.0;
+  // from u = 1 on no sum exceeds it: a partial sum may round above a total that was added in another order
+  const double level = u > 0.f ? (u < 1.f ? static_cast<double>(u) * total : __builtin_inf()) : 0.0;
   // the first run of the stretch behind which the sum exceeds the level, and the last with weight
   int64_t hit = -1, last = -1;
   double run = upto - mine, at_hit = 0.0, at_last = 0.0;

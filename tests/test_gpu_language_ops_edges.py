@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import language_ops as L
-from tests.test_gpu_language_ops import DTYPES, _distill_case, _run_distill, ws  # noqa: F401
+from tests.test_gpu_language_ops import DTYPES, _distill_case, _run_distill, _run_verify, ws  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -226,3 +226,21 @@ def test_operator_rms_norm_gradient_of_other_rows_than_the_forward_saw(ws):
     for other in ("more", "less"):
         with pytest.raises(rt.DragonError, match="other rows"):
             ws.run_operator(text.replace('input: "x"', 'input: "%s"' % other))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("C", [700, 32000, 70001])
+def test_draft_verify_at_the_end_of_the_running_sum(dtype, C):
+    """u = 1 and more draw the last class of non-zero weight, however the sums round: the last weights here are far
+    below half a step of the total."""
+    B = 64
+    rng = np.random.default_rng(C)
+    p = rng.random((B, 1, C)) ** 4
+    p[:, :, C - 40:] = 0
+    p[:, :, C - 3] = 1e-25
+    for u in (1.0, 1.5, np.inf):
+        t = {"target": torch.from_numpy(p).to(getattr(torch, dtype)).cuda(), "draft": None,
+             "drafted": torch.zeros((B, 0), dtype=torch.int64, device="cuda"), "lengths": None,
+             "u_accept": torch.zeros((B, 0), device="cuda"), "u_sample": torch.full((B,), u, device="cuda")}
+        tokens, accepted = _run_verify(t)
+        assert (tokens == C - 3).all() and not accepted.any(), u
