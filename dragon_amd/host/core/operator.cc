@@ -80,6 +80,19 @@ Tensor& OperatorBase::Input(const string& name) { return *ws_->GetTensor(handle_
 
 Tensor* OperatorBase::Output(const string& name) { return ws_->CreateTensor(handle_ + "/" + name); }
 
+void OperatorBase::CheckOutputsApart() const {
+  for (size_t i = 0; i < outputs_.size(); ++i) {
+    for (size_t j = 0; j < inputs_.size(); ++j) {
+      CHECK(outputs_[i] != inputs_[j]) << "\nOperator(" << type() << "): Output(" << i << ") is the tensor of Input("
+                                       << j << "): " << outputs_[i]->name();
+    }
+    for (size_t j = 0; j < i; ++j) {
+      CHECK(outputs_[i] != outputs_[j]) << "\nOperator(" << type() << "): Output(" << i
+                                        << ") is the tensor of Output(" << j << "): " << outputs_[i]->name();
+    }
+  }
+}
+
 string OperatorBase::MessageForUnsupported(const string& value, const vector<string>& support) const {
   std::stringstream ss;
   ss << "Unsupported type of Operator(" << type() << "): " << value << "\n<" << type()

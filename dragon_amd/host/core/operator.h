@@ -58,6 +58,10 @@ class OperatorBase {
   const OperatorDef& def() const { return def_; }
   Workspace* workspace() const { return ws_; }
   void SwitchToPhase(const string& phase) { phase_ = phase; }
+  // For operators whose outputs differ in type or size from each other and from the inputs: an output that is
+  // an input's tensor, or another output's, would take the memory away that the kernel is to use. The schema
+  // looks at the definition that an operator is created from; this also at what a cached one is rebound to.
+  void CheckOutputsApart() const;
 
   string MessageForUnsupported(const string& value, const vector<string>& support) const;
 

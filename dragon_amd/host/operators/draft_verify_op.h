@@ -19,6 +19,7 @@ class DraftVerifyOp final : public Operator<Context> {
   DraftVerifyOp(const OperatorDef& def, Workspace* ws) : Operator<Context>(def, ws) {}
   USE_OPERATOR_FUNCTIONS;
 
+  void Setup() override { this->CheckOutputsApart(); }
   void RunOnDevice() override { FloatingDispatch::Call(this, Input(0)); }
 
   template <typename T>

@@ -25,6 +25,7 @@ namespace dragon {
           epsilon_(OP_SINGLE_ARG(double, "epsilon", 1e-5)),                                     \
           group_size_(OP_SINGLE_ARG(int64_t, "group_size", 0)) {}                               \
     USE_OPERATOR_FUNCTIONS;                                                                     \
+    void Setup() override { this->CheckOutputsApart(); }                                        \
     void RunOnDevice() override { Dispatch::Call(this, Input(0)); }                             \
     template <typename T>                                                                       \
     void DoRunWithType();                                                                       \

@@ -24,6 +24,7 @@ namespace dragon {
           temperature_(OP_SINGLE_ARG(float, "temperature", 1.f)),             \
           reduction_(OP_SINGLE_ARG(string, "reduction", "VALID")) {}          \
     USE_OPERATOR_FUNCTIONS;                                                   \
+    void Setup() override { this->CheckOutputsApart(); }                      \
     void RunOnDevice() override { FloatingDispatch::Call(this, Input(0)); }   \
     template <typename T>                                                     \
     void DoRunWithType();                                                     \

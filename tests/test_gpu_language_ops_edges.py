@@ -244,3 +244,15 @@ def test_draft_verify_at_the_end_of_the_running_sum(dtype, C):
              "u_accept": torch.zeros((B, 0), device="cuda"), "u_sample": torch.full((B,), u, device="cuda")}
         tokens, accepted = _run_verify(t)
         assert (tokens == C - 3).all() and not accepted.any(), u
+
+
+def test_operator_rms_norm_of_a_tensor_that_is_its_own_residual(ws):
+    """The sum is right; its gradient would be two shares in one tensor, and is refused."""
+    from dragon_amd import runtime as rt
+    ws.feed("x", np.arange(8, dtype=np.float32).reshape(2, 4))
+    ws.feed("w", np.ones(4, np.float32))
+    tape = rt.Tape(ws)
+    y, h = rt.rms_norm(tape, ["x", "w", "x"])
+    assert np.array_equal(ws.fetch(h), 2 * ws.fetch("x"))
+    with pytest.raises(rt.DragonError, match=r"Output\(2\) is the tensor of Output\(0\)"):
+        tape.gradient(y, ["x"], output_gradient=h)

@@ -178,6 +178,35 @@ def test_gradient_definitions_of_rms_norm_by_what_arrives(ws):
     assert "RMSNormSumGradient" in rt.registered_operators()
 
 
+@pytest.mark.parametrize("op,inputs,outputs", [
+    ("RMSNorm", "xwr", "yy"), ("RMSNormQuant", "xw", "qq"), ("RMSNormQuant", "xwr", "qsq"), ("RMSNormGradient", "xwr", "aa"),
+    ("RMSNormGradient", "xwr", "aba"), ("RMSNormSumGradient", "xw", "aba"), ("DraftVerify", "xiirr", "tt")])
+def test_operators_refuse_one_tensor_for_two_outputs(ws, op, inputs, outputs):
+    """They differ in type or size: the second would free the memory that was taken for the first. Refused before
+    the device is looked at."""
+    from dragon_amd import runtime as rt
+    for n, dtype in (("x", np.float32), ("w", np.float32), ("r", np.float32), ("i", np.int64)):
+        ws.feed(n, np.zeros(8, dtype))
+    with pytest.raises(rt.DragonError, match=r"Output\(\d\) is the tensor of Output\(0\)"):
+        ws.run_operator(rt.make_def(op, list(inputs), list(outputs)))
+
+
+@pytest.mark.parametrize("op,inputs,outputs", [("RMSNorm", "xw", "y"), ("RMSNormQuant", "xw", "qs"), ("RMSNormSumGradient", "xw", "abc"),
+                                               ("TopKDistillationLoss", "xir", "l"), ("DraftVerify", "xiirr", "ta")])
+def test_cached_operators_refuse_an_input_for_an_output(ws, op, inputs, outputs):
+    """The schema refuses it of a new operator; one that is rebound to other tensors says so too."""
+    from dragon_amd import runtime as rt
+    for n, dtype in (("x", np.float32), ("w", np.float32), ("r", np.float32), ("i", np.int64)):
+        ws.feed(n, np.zeros(8, dtype))
+    define = lambda out: rt.make_def(op, list(inputs), out, cache_key="k")
+    try:
+        ws.run_operator(define(list(outputs)))
+    except rt.DragonError:
+        pass  # it is created; without a device, or with shapes that do not fit, it does not run
+    with pytest.raises(rt.DragonError, match=r"Output\(0\) is the tensor of Input\(0\)"):
+        ws.run_operator(define([inputs[0]] + list(outputs[1:])))
+
+
 # ---------------------------------------------------------------- the plain forms themselves
 
 def test_plain_distillation_is_the_divergence_of_torch():
