@@ -454,13 +454,21 @@ int launch_verify(int64_t B, int64_t K, int64_t C, const void* target, const voi
   IndexT* op = static_cast<IndexT*>(tokens);
   IndexT* ap = static_cast<IndexT*>(accepted);
   const PartPlan plan = plan_parts<T>(B, C);
+  const size_t need = plan.parts == 0 ? 0 : static_cast<size_t>(B * plan.row_runs) * sizeof(double);
+  // several workgroups read the inputs of a sequence whose outputs one of them writes
+  const Span P = {target, bytes_of(sizeof(T), B, K + 1, C)}, Q = {draft, bytes_of(sizeof(T), B, K, C)};
+  const Span D = {drafted, bytes_of(sizeof(IndexT), B, K)}, L = {lengths, bytes_of(sizeof(IndexT), B)};
+  const Span U = {u_accept, bytes_of(4, B, K)}, V = {u_sample, bytes_of(4, B)};
+  const Span O = {tokens, bytes_of(sizeof(IndexT), B, K + 1)}, N = {accepted, bytes_of(sizeof(IndexT), B)};
+  const Span W = {scratch, need};
+  if (!apart(O, {P, Q, D, L, U, V, N}) || !apart(N, {P, Q, D, L, U, V}) || !apart(W, {P, Q, D, L, U, V, O, N}))
+    return DRAGON_HIP_EINVAL;
   if (plan.parts == 0) {
     hipLaunchKernelGGL((draft_verify_rows<T, IndexT>), dim3(row_grid(B, 1)), dim3(rows_waves<T>() * kWaveSize), 0,
                        stream, B, K, C, tp, qp, dp, lp, ua, us, op, ap);
   } else {
     double* sums = static_cast<double*>(scratch);
-    if (!sums || scratch_bytes < static_cast<size_t>(B * plan.row_runs) * sizeof(double))
-      return DRAGON_HIP_ESCRATCH;
+    if (!sums || scratch_bytes < need) return DRAGON_HIP_ESCRATCH;
     const dim3 block(kPartWaves * kWaveSize);
     hipLaunchKernelGGL((draft_verify_runs<T, IndexT>), dim3(row_grid(B * plan.parts, 1)), block, 0, stream,
                        B, K, C, static_cast<uint32_t>(plan.parts), plan.part_runs, plan.row_runs, tp, qp, dp,
@@ -516,12 +524,6 @@ int dragon_hip_draft_verify(int dtype, int index_dtype, int64_t B, int64_t K, in
   if (B < 0 || B > INT_MAX || K < 0 || K >= INT_MAX || C <= 0 || C > INT_MAX) return DRAGON_HIP_EINVAL;
   if (B == 0) return DRAGON_HIP_OK;
   if (!target || !u_sample || !tokens || !accepted || (K > 0 && (!drafted || !u_accept)))
-    return DRAGON_HIP_EINVAL;
-  // several workgroups read the inputs of a sequence whose outputs one of them writes
-  const uint64_t one = index_dtype == DRAGON_HIP_I32 ? 4 : 8, each = B * one, all = each * K;
-  if (overlaps(accepted, each, lengths, each) || overlaps(accepted, each, drafted, all) ||
-      overlaps(tokens, all + each, drafted, all) || overlaps(tokens, all + each, lengths, each) ||
-      overlaps(tokens, all + each, accepted, each))
     return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_DTYPE(dtype, launch_verify_index, index_dtype, B, K, C, target, draft, drafted,

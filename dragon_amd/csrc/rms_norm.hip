@@ -836,7 +836,14 @@ int launch_rms_norm_grad(int64_t N, int64_t C, const void* h, const void* rsig, 
                          const void* dy, const void* dh, void* dgamma, void* dx, void* scratch,
                          size_t scratch_bytes, hipStream_t stream) {
   using A = typename IO<T>::Acc;
-  if (N > 0 && (!scratch || scratch_bytes < grad_scratch_bytes<T>(N, C))) return DRAGON_HIP_ESCRATCH;
+  const size_t need = N > 0 ? grad_scratch_bytes<T>(N, C) : 0;
+  const uint64_t bytes = bytes_of(sizeof(T), N, C);
+  const Span H = {h, bytes}, S = {rsig, bytes_of(sizeof(A), N)}, G = {gamma, bytes_of(sizeof(A), C)}, DY = {dy, bytes};
+  const Span DH = {dh, bytes}, DG = {dgamma, bytes_of(sizeof(A), C)}, DX = {dx, bytes}, W = {scratch, need};
+  if (!on_or_apart(DX, {DY, DH}) || !apart(DX, {H, S, G}) || !apart(DG, {H, S, G, DY, DH, DX}) ||
+      !apart(W, {H, S, G, DY, DH, DG, DX}))
+    return DRAGON_HIP_EINVAL;
+  if (need > 0 && (!scratch || scratch_bytes < need)) return DRAGON_HIP_ESCRATCH;
   const T* hp = static_cast<const T*>(h);
   const T* yp = static_cast<const T*>(dy);
   const T* dp = static_cast<const T*>(dh);
@@ -874,6 +881,7 @@ int launch_rms_norm_grad(int64_t N, int64_t C, const void* h, const void* rsig, 
 inline int element_bytes(int dtype) {
   return dtype == DRAGON_HIP_F64 ? 8 : (dtype == DRAGON_HIP_F32 ? 4 : 2);
 }
+inline int acc_bytes(int dtype) { return dtype == DRAGON_HIP_F64 ? 8 : 4; }
 inline bool sizes_ok(int64_t N, int64_t C) { return N >= 0 && C > 0 && N <= INT_MAX && C <= INT_MAX; }
 
 } // namespace
@@ -888,9 +896,12 @@ int dragon_hip_rms_norm(int dtype, int64_t N, int64_t C, float eps, const void* 
                         void* stream) {
   if (!sizes_ok(N, C)) return DRAGON_HIP_EINVAL;
   if (N == 0) return DRAGON_HIP_OK;
-  const uint64_t bytes = static_cast<uint64_t>(N) * C * element_bytes(dtype);
-  if (!x || !gamma || !y || overlaps(y, bytes, h, bytes)) return DRAGON_HIP_EINVAL;
-  if (across(y, x, bytes) || across(y, residual, bytes) || across(h, x, bytes) || across(h, residual, bytes))
+  const uint64_t bytes = bytes_of(element_bytes(dtype), N, C);
+  if (!x || !gamma || !y) return DRAGON_HIP_EINVAL;
+  const Span X = {x, bytes}, R = {residual, bytes}, G = {gamma, bytes_of(acc_bytes(dtype), C)};
+  const Span H = {h, bytes}, S = {rsig, bytes_of(acc_bytes(dtype), N)}, Y = {y, bytes};
+  if (!on_or_apart(Y, {X, R}) || !on_or_apart(H, {X, R}) || !apart(Y, {H, G, S}) || !apart(H, {G, S}) ||
+      !apart(S, {X, R, G}))
     return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_DTYPE(dtype, launch_rms_norm, N, C, eps, x, residual, gamma, h, rsig, y, s);
@@ -905,9 +916,12 @@ int dragon_hip_rms_norm_quant(int dtype, int64_t N, int64_t C, int64_t group, fl
   if (group != 0 && group != 32 && group != 64 && group != 128 && group != 256) return DRAGON_HIP_EINVAL;
   if (N == 0) return DRAGON_HIP_OK;
   if (!x || !gamma || !q || !scale) return DRAGON_HIP_EINVAL;
-  const uint64_t codes = static_cast<uint64_t>(N) * C, bytes = codes * element_bytes(dtype);
-  if (across(h, x, bytes) || across(h, residual, bytes) || overlaps(q, codes, x, bytes) ||
-      overlaps(q, codes, residual, bytes) || overlaps(q, codes, h, bytes))
+  const uint64_t bytes = bytes_of(element_bytes(dtype), N, C);
+  const Span X = {x, bytes}, R = {residual, bytes}, G = {gamma, bytes_of(4, C)}, H = {h, bytes};
+  const Span S = {rsig, bytes_of(4, N)}, Q = {q, bytes_of(1, N, C)};
+  const Span scales = {scale, bytes_of(4, N, group ? ceil_div(C, group) : 1)};
+  if (!on_or_apart(H, {X, R}) || !apart(H, {G, S}) || !apart(S, {X, R, G}) || !apart(Q, {X, R, G, H, S}) ||
+      !apart(scales, {X, R, G, H, S, Q}))
     return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
@@ -936,9 +950,6 @@ int dragon_hip_rms_norm_grad(int dtype, int64_t N, int64_t C, const void* h, con
                              void* dx, void* scratch, size_t scratch_bytes, void* stream) {
   if (!sizes_ok(N, C)) return DRAGON_HIP_EINVAL;
   if (!dgamma || (N > 0 && (!h || !rsig || !gamma || !dy || !dx))) return DRAGON_HIP_EINVAL;
-  const uint64_t bytes = static_cast<uint64_t>(N) * C * element_bytes(dtype);
-  if (N > 0 && (overlaps(dx, bytes, h, bytes) || across(dx, dy, bytes) || across(dx, dh, bytes)))
-    return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_DTYPE(dtype, launch_rms_norm_grad, N, C, h, rsig, gamma, dy, dh, dgamma, dx,
                             scratch, scratch_bytes, s);

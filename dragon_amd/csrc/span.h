@@ -1,7 +1,9 @@
 // Pieces of rows at any alignment, shared by the kernels that walk rows packet
 // by packet: up to kVec elements from an element-aligned address. And the host's
-// check that an output does not lie across a tensor.
+// checks of which tensors share memory.
 #pragma once
+
+#include <initializer_list>
 
 #include "common.h"
 
@@ -38,14 +40,37 @@ __device__ __forceinline__ void store_span(T* p, int n, const typename IO<T>::Ac
   }
 }
 
-// Whether two tensors of so many bytes share memory; a null pointer is no tensor.
-inline bool overlaps(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
-  return p && q && p < q + b_bytes && q < p + a_bytes;
+// A tensor's memory, as the host's checks of arguments see it; a null pointer is no tensor.
+struct Span {
+  const void* p;
+  uint64_t bytes;
+};
+// Bytes of a tensor of these extents (none negative), or more than any memory holds.
+inline uint64_t bytes_of(uint64_t element, int64_t a, int64_t b = 1, int64_t c = 1) {
+  uint64_t n = element;
+  for (const int64_t extent : {a, b, c}) {
+    if (__builtin_mul_overflow(n, static_cast<uint64_t>(extent), &n)) return UINT64_MAX;
+  }
+  return n;
 }
-// Whether an output shares memory with an input of its size without being the very buffer of it.
-inline bool across(const void* out, const void* in, uint64_t bytes) {
-  return out != in && overlaps(out, bytes, in, bytes);
+inline bool overlap(const Span& a, const Span& b) {
+  if (!a.p || !b.p || a.bytes == 0 || b.bytes == 0) return false;
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a.p), q = reinterpret_cast<uintptr_t>(b.p);
+  return p <= q ? q - p < a.bytes : p - q < b.bytes;
+}
+// Whether an output shares memory with none of the others.
+inline bool apart(const Span& out, std::initializer_list<Span> others) {
+  for (const Span& other : others) {
+    if (overlap(out, other)) return false;
+  }
+  return true;
+}
+// Whether an output is the very buffer of each of these inputs of its size, or shares nothing with it.
+inline bool on_or_apart(const Span& out, std::initializer_list<Span> inputs) {
+  for (const Span& in : inputs) {
+    if (out.p != in.p && overlap(out, in)) return false;
+  }
+  return true;
 }
 
 } // namespace dragon_hip

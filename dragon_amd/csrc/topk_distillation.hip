@@ -788,6 +788,18 @@ inline bool sizes_ok(int64_t N, int64_t C, int64_t K, float temperature, float n
       temperature < 1e18f && normalizer == normalizer;
 }
 
+// What both calls are given; `loss` is the loss or its gradient.
+struct Tensors {
+  Span x, index, teacher, stats, loss;
+};
+inline Tensors tensors_of(int dtype, int index_dtype, int64_t N, int64_t C, int64_t K, const void* x, const void* index,
+                          const void* teacher, const void* stats, const void* loss, float normalizer) {
+  const int element = dtype == DRAGON_HIP_F64 ? 8 : (dtype == DRAGON_HIP_F32 ? 4 : 2);
+  const int acc = dtype == DRAGON_HIP_F64 ? 8 : 4, one = index_dtype == DRAGON_HIP_I32 ? 4 : 8;
+  return {{x, bytes_of(element, N, C)}, {index, bytes_of(one, N, K)}, {teacher, bytes_of(acc, N, K)},
+          {stats, bytes_of(acc, N + 1)}, {loss, bytes_of(acc, normalizer == 0.f ? N : 1)}};
+}
+
 // Calls FN<T, IndexT>(args...).
 #define DRAGON_HIP_DISPATCH_INDEXED(dtype, index_dtype, FN, ...)                    \
   switch (dtype) {                                                                  \
@@ -831,6 +843,11 @@ int dragon_hip_topk_distillation_loss_forward(int dtype, int index_dtype, int64_
     return DRAGON_HIP_EINVAL;
   const size_t need = dragon_hip_topk_distillation_loss_scratch_bytes(dtype, N, C);
   if (need > 0 && (!scratch || scratch_bytes < need)) return DRAGON_HIP_ESCRATCH;
+  const Tensors t = tensors_of(dtype, index_dtype, N, C, K, x, index, teacher, stats, loss, normalizer);
+  const Span W = {scratch, need};
+  if (!apart(t.stats, {t.x, t.index, t.teacher, t.loss}) || !apart(t.loss, {t.x, t.index, t.teacher}) ||
+      !apart(W, {t.x, t.index, t.teacher, t.stats, t.loss}))
+    return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_INDEXED(dtype, index_dtype, launch_forward, N, C, K, temperature, normalizer, x,
                               index, teacher, stats, loss, scratch, s);
@@ -845,8 +862,9 @@ int dragon_hip_topk_distillation_loss_backward(int dtype, int index_dtype, int64
   if (!sizes_ok(N, C, K, temperature, normalizer)) return DRAGON_HIP_EINVAL;
   if (N == 0) return DRAGON_HIP_OK;
   if (!x || !index || !teacher || !stats || !dl || !dx) return DRAGON_HIP_EINVAL;
-  const int element = dtype == DRAGON_HIP_F64 ? 8 : (dtype == DRAGON_HIP_F32 ? 4 : 2);
-  if (across(dx, x, static_cast<uint64_t>(N) * C * element)) return DRAGON_HIP_EINVAL;
+  const Tensors t = tensors_of(dtype, index_dtype, N, C, K, x, index, teacher, stats, dl, normalizer);
+  const Span DX = {dx, t.x.bytes};
+  if (!on_or_apart(DX, {t.x}) || !apart(DX, {t.index, t.teacher, t.stats, t.loss})) return DRAGON_HIP_EINVAL;
   hipStream_t s = static_cast<hipStream_t>(stream);
   DRAGON_HIP_DISPATCH_INDEXED(dtype, index_dtype, launch_backward, N, C, K, temperature, normalizer, x,
                               index, teacher, stats, dl, dx, s);

@@ -256,3 +256,38 @@ def test_operator_rms_norm_of_a_tensor_that_is_its_own_residual(ws):
     assert np.array_equal(ws.fetch(h), 2 * ws.fetch("x"))
     with pytest.raises(rt.DragonError, match=r"Output\(2\) is the tensor of Output\(0\)"):
         tape.gradient(y, ["x"], output_gradient=h)
+
+
+def test_tensors_side_by_side_are_taken():
+    """Outputs that end where inputs begin, and the other way round, share nothing."""
+    from dragon_amd import kernels as K
+    flat = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    at = 0
+    def carve(shape, dtype):
+        nonlocal at
+        n = int(np.prod(shape)) * torch.empty((), dtype=dtype).element_size()
+        t = flat[at:at + n].view(dtype).view(shape)
+        at += n
+        return t
+    f, b, i64 = torch.float32, torch.bfloat16, torch.int64
+    N, C = 4, 64
+    x, h, r, y = carve((N, C), f), carve((N, C), f), carve((N, C), f), carve((N, C), f)
+    g, rsig, dg = carve((C,), f), carve((N,), f), carve((C,), f)
+    q, scale = carve((N, C), torch.uint8), carve((N, 2), f)
+    x.normal_(), r.normal_(), g.fill_(1)
+    K.rms_norm(N, C, 1e-5, x, r, g, h, rsig, y)
+    K.rms_norm_quant(N, C, 32, 1e-5, x, r, g, h, rsig, q, scale)
+    K.rms_norm_grad(N, C, h, rsig, g, x, r, dg, y)
+    at = (at + 7) // 8 * 8
+    index, teacher, stats, loss, dl = carve((N, 2), i64), carve((N, 2), f), carve((N + 1,), f), carve((1,), f), carve((1,), f)
+    K.topk_distillation_loss_forward(N, C, 2, 1.0, "MEAN", x, index, teacher, stats, loss)
+    K.topk_distillation_loss_backward(N, C, 2, 1.0, "MEAN", x, index, teacher, stats, dl, h)
+    at = (at + 7) // 8 * 8
+    B, k = 2, 3
+    target, tokens, draft = carve((B, k + 1, 16), f), carve((B, k + 1), i64), carve((B, k, 16), f)
+    accepted, drafted, lengths = carve((B,), i64), carve((B, k), i64), carve((B,), i64)
+    ua, us = carve((B, k), f), carve((B,), f)
+    target.fill_(1 / 16)
+    K.draft_verify(B, k, 16, target, draft, drafted, lengths, ua, us, tokens, accepted)
+    torch.cuda.synchronize()
+    assert torch.isfinite(flat[:at // 4 * 4].view(f)[:4 * N * C]).all()

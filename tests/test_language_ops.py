@@ -77,6 +77,57 @@ def test_outputs_that_lie_across_inputs_are_refused():
     assert verify(acc=at(P[2], 8)) == EINVAL and verify(acc=at(P[6], 56)) == EINVAL
 
 
+def _shared(call, tensors, outputs, very=()):
+    """Lays each output over every other tensor: on its first byte, on its last, with its own last byte on the
+    first. (output, input) pairs in `very` may be one buffer. tensors: name -> bytes."""
+    at = {n: (i + 1) << 32 for i, n in enumerate(tensors)}
+    for out in outputs:
+        for other in tensors:
+            if other == out:
+                continue
+            for shift in (0, tensors[other] - 1, 1 - tensors[out]):
+                if shift == 0 and ((out, other) in very or (other, out) in very):
+                    continue
+                place = dict(at, **{out: at[other] + shift})
+                assert call(*[ctypes.c_void_p(place[n]) for n in tensors]) == EINVAL, (out, other, shift)
+
+
+def test_no_output_shares_memory_with_another_tensor():
+    """Every output against every other tensor of the call, scratch among them."""
+    lib = _lib.lib()
+    N, C, k = 6, 40, 3
+    for dtype, e, a in ((1, 2, 4), (2, 4, 4), (3, 8, 8)):
+        n = N * C * e
+        _shared(lambda x, r, g, h, rs, y: lib.dragon_hip_rms_norm(dtype, N, C, 1e-5, x, r, g, h, rs, y, None),
+                dict(x=n, r=n, g=C * a, h=n, rs=N * a, y=n), ("h", "rs", "y"), [(o, i) for o in "hy" for i in "xr"])
+        if dtype != 3:
+            for group, groups in ((0, 1), (32, 2)):
+                _shared(lambda x, r, g, h, rs, q, s: lib.dragon_hip_rms_norm_quant(dtype, N, C, group, 1e-5, x, r, g, h, rs, q, s, None),
+                        dict(x=n, r=n, g=C * a, h=n, rs=N * a, q=N * C, s=N * groups * 4), ("h", "rs", "q", "s"), [("h", "x"), ("h", "r")])
+        need = lib.dragon_hip_rms_norm_grad_scratch_bytes(dtype, N, C)
+        _shared(lambda h, rs, g, dy, dh, dg, dx, ws: lib.dragon_hip_rms_norm_grad(dtype, N, C, h, rs, g, dy, dh, dg, dx, ws, need, None),
+                dict(h=n, rs=N * a, g=C * a, dy=n, dh=n, dg=C * a, dx=n, ws=need), ("dg", "dx", "ws"), [("dx", "dy"), ("dx", "dh")])
+        for it, one in ((4, 4), (5, 8)):
+            for norm, losses in ((0.0, N), (-1.0, 1)):
+                need = lib.dragon_hip_topk_distillation_loss_scratch_bytes(dtype, N, C)
+                _shared(lambda x, i, t, st, l, ws: lib.dragon_hip_topk_distillation_loss_forward(
+                            dtype, it, N, C, k, 1.0, norm, x, i, t, st, l, ws, need, None),
+                        dict(x=n, i=N * k * one, t=N * k * a, st=(N + 1) * a, l=losses * a, ws=need), ("st", "l", "ws"))
+                _shared(lambda x, i, t, st, dl, dx: lib.dragon_hip_topk_distillation_loss_backward(
+                            dtype, it, N, C, k, 1.0, norm, x, i, t, st, dl, dx, None),
+                        dict(x=n, i=N * k * one, t=N * k * a, st=(N + 1) * a, dl=losses * a, dx=n), ("dx",), [("dx", "x")])
+            for B, V in ((2, 40), (2, 40000)):  # in one launch, and in two with scratch
+                need = lib.dragon_hip_draft_verify_scratch_bytes(dtype, B, k, V)
+                assert (need > 0) == (V > 32768)
+                sizes = dict(p=B * (k + 1) * V * e, q=B * k * V * e, d=B * k * one, n=B * one, ua=B * k * 4, us=B * 4,
+                             tok=B * (k + 1) * one, acc=B * one)
+                if need:
+                    sizes["ws"] = need
+                call = lambda p, q, d, n, ua, us, tok, acc, ws=None: lib.dragon_hip_draft_verify(
+                    dtype, it, B, k, V, p, q, d, n, ua, us, tok, acc, ws, need, None)
+                _shared(call, sizes, ("tok", "acc") + (("ws",) if need else ()))
+
+
 def test_distillation_refusals():
     lib = _lib.lib()
     fwd = lambda dtype=1, it=5, N=4, C=8, k=2, t=1.0, norm=-1.0, x=P[0], st=P[3], loss=P[4], ws=P[5], nbytes=BIG: \
