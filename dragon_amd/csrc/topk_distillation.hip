@@ -23,7 +23,9 @@ constexpr int kMaxK = 1024;  // entries that a workgroup holds
 // that running maxima m are held in; term(x) is exp of the logit x relative to m, shrink(d) the
 // factor that a maximum which grows by -d leaves to a sum.
 //   16-bit logits: the base-2 domain, one fused multiply-add and the hardware's exp2 per element.
-//   The roundings of scale and m move a term by parts in 10^6, a thousandth of a logit's own.
+//   The rounding of scale moves a term by 2^-24 of its logit's distance from the maximum, that of m all
+//   terms alike, by 2^-24 |m| log 2 (8e-5 at most, below kFar); the loss adds distances from the rounded m,
+//   in which that cancels.
 //   32-bit logits: the natural domain, so that the argument of the largest terms, near 0, is
 //   exact to its last bits; then exp2. 64-bit logits: the library's exp.
 template <typename T>
@@ -66,7 +68,9 @@ struct ExpMath {
 // maximum itself is exp of that rounding, a part in 10^4 at 2048 and anything from 0 to infinity at
 // the lowest value of a type, which masks are made of. The floor keeps masked stretches of a row
 // (threads, segments) at sums of 0. Rows whose maximum is not inside (-kFar, kFar) are masked all
-// over, or are logits of unusual size: they are read again by far_sum, which subtracts first.
+// over, or are logits of unusual size: they are read again by far_sum, which subtracts first. In the domain of
+// m: 16-bit logits are held in base 2, where kFar is 1420 in x / t. The gradient, which has no maximum, goes by the
+// log-sum, and by half of kFar.
 constexpr int kFar = 2048;
 template <typename A>
 struct ExpSum {

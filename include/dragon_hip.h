@@ -350,10 +350,12 @@ int dragon_hip_softmax_cross_entropy_loss_backward(int dtype, int target_dtype, 
 /* RMSNorm of s = x + residual (residual may be NULL: s = x), per row of C:
  *   rsig = 1 / sqrt(mean(s^2) + eps),  y = s * rsig * gamma,  h = s
  * x, residual, y, h: T[N, C]; gamma: AccT[C]; rsig: AccT[N]. s is held in AccT
- * and rounded once into h and once into y. h and rsig may be NULL where the
- * caller has no use for them. Each output may be the very buffer of x or of
- * residual (y and h may not be the same buffer); memory shared in any other way
- * is refused, here and in the calls below. N and C below 2^31. */
+ * and rounded once into h and once into y; a row whose sum of squares is beyond
+ * AccT's range has rsig 0. h and rsig may be NULL where the caller has no use for
+ * them. y and h may each be the very buffer of x or of residual (not both of one).
+ * Here and in the calls below an output, or scratch, that shares memory with
+ * another tensor of the call in a way that is not named is refused
+ * (DRAGON_HIP_EINVAL). N and C below 2^31. */
 int dragon_hip_rms_norm(int dtype, int64_t N, int64_t C, float eps, const void* x,
                         const void* residual, const void* gamma, void* h, void* rsig, void* y,
                         void* stream);
@@ -362,9 +364,12 @@ int dragon_hip_rms_norm(int dtype, int64_t N, int64_t C, float eps, const void* 
  * consecutive columns of a row (32, 64, 128 or 256; 0: the whole row is one
  * group; the last group of a row may be shorter):
  *   scale = max(max|y|, 1e-30) / 448,  q = e4m3(y / scale)
- * q: one byte per element [N, C], apart from x, residual and h; scale: float[N, ceil(C / group)]. A NaN in y
- * becomes a NaN code and is passed over by the maximum; an infinity makes its
- * group's scale infinite. dtype F16, BF16 or F32 (DRAGON_HIP_EDTYPE otherwise). */
+ * formed as y * (448 / max|y|) in 32 bits, whose two roundings decide between the
+ * neighbours of a quotient that lies on the border of two codes.
+ * q: one byte per element [N, C]; scale: float[N, ceil(C / group)]; h may be the
+ * very buffer of x or of residual. A NaN in y becomes a NaN code and is passed over
+ * by the maximum; an infinity makes its group's scale infinite.
+ * dtype F16, BF16 or F32 (DRAGON_HIP_EDTYPE otherwise). */
 int dragon_hip_rms_norm_quant(int dtype, int64_t N, int64_t C, int64_t group, float eps,
                               const void* x, const void* residual, const void* gamma, void* h,
                               void* rsig, void* q, void* scale, void* stream);
@@ -391,10 +396,14 @@ int dragon_hip_rms_norm_grad(int dtype, int64_t N, int64_t C, const void* h, con
  * listed; a class that is listed twice receives both shares. A row that lists
  * nothing is ignored: its loss and gradient are 0 whatever its logits hold, and
  * it is not read. A row whose logits are all -inf, or that holds NaN or +inf,
- * has a NaN loss and NaN gradients.
- * Loss and gradient hold for logits of any size, rows masked all over by the
- * type's lowest value among them; rows whose log-sum is beyond +-1024 are read
- * two times more (the log-sum, a single AccT, no longer holds the sum).
+ * has a NaN loss and NaN gradients; one that lists a teacher logit of NaN or +inf
+ * a NaN loss and NaN gradients at its listed classes.
+ * Loss and gradient hold for logits of any size on both sides, rows masked all over
+ * by the type's lowest value among them. The forward reads a row two times more
+ * where its largest x / t is not inside (-2048, 2048) (16-bit dtypes: 2048 log 2 =
+ * 1419.6, in base 2), the gradient where its log-sum is beyond +-1024: a single AccT
+ * holds the log-sum, to half a step, by which the softmax of the gradient is off
+ * (up to 8e-5 of itself below 1024 in 32 bits).
  * normalizer: 0 keeps a loss per row (loss: AccT[N], dl: AccT[N]); otherwise
  * loss = sum of rows / max(divisor, 1) (AccT[1], dl: AccT[1], the gradient
  * divides by max(divisor, 0.5), as ReduceLossGrad) with divisor = normalizer,
@@ -432,7 +441,7 @@ int dragon_hip_topk_distillation_loss_backward(int dtype, int index_dtype, int64
  * tokens (index type, [B, K + 1]) = the n accepted, the sampled one, -1 behind it;
  * accepted (index type, [B]) = n. Probabilities that are negative or not finite count as 0; a
  * drafted token outside [0, C) is refused. Comparisons and sums are held in 64 bits. K may be
- * 0 (draft, drafted, u_accept unused). B, K and C below 2^31. No output may lie on an input. */
+ * 0 (draft, drafted, u_accept unused). B, K and C below 2^31. */
 size_t dragon_hip_draft_verify_scratch_bytes(int dtype, int64_t B, int64_t K, int64_t C);
 int dragon_hip_draft_verify(int dtype, int index_dtype, int64_t B, int64_t K, int64_t C,
                             const void* target, const void* draft, const void* drafted,

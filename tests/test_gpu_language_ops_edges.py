@@ -291,3 +291,21 @@ def test_tensors_side_by_side_are_taken():
     K.draft_verify(B, k, 16, target, draft, drafted, lengths, ua, us, tokens, accepted)
     torch.cuda.synchronize()
     assert torch.isfinite(flat[:at // 4 * 4].view(f)[:4 * N * C]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C,k", [(130, 4), (9001, 70), (70001, 5)])
+def test_distillation_of_teacher_logits_that_are_not_finite(dtype, C, k):
+    """NaN or +inf among a row's listed teacher logits: no loss, and no gradient at the listed classes; the other
+    classes' and the other rows' are those of a teacher without it."""
+    x, _, teacher = _distill_case(4, C, k, dtype, torch.int64, 6)
+    teacher.nan_to_num_(neginf=0.0)
+    index = torch.stack([torch.randperm(C)[:k] for _ in range(4)]).cuda()
+    dl = torch.full((4,), 0.5, dtype=teacher.dtype, device="cuda")
+    stats, loss, dx = _run_distill(x, index, teacher, 1.5, "NONE", dl)
+    teacher[1, 2], teacher[3, k - 1] = float("nan"), float("inf")
+    got = _run_distill(x, index, teacher, 1.5, "NONE", dl)
+    assert torch.equal(got[0], stats) and torch.equal(got[1][::2], loss[::2]) and got[1][1::2].isnan().all()
+    listed = torch.zeros((4, C), dtype=torch.bool, device="cuda").scatter_(1, index, True)
+    listed[::2] = False
+    assert got[2][listed].isnan().all() and torch.equal(got[2][~listed], dx[~listed])
