@@ -305,6 +305,8 @@ def broadcast_loss_grad(N, S, C, dl, dx):
 
 # ---------------------------------------------------------------- operators of language models
 
+# Outputs share no memory with each other or with inputs but where a function says so; the library refuses it.
+
 _BYTE_DTYPES = (torch.uint8, torch.float8_e4m3fn)
 _ACC_DTYPES = {0: torch.float32, 1: torch.float32, 2: torch.float32, 3: torch.float64}
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
