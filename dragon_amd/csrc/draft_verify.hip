@@ -429,7 +429,7 @@ __global__ __launch_bounds__(kPartWaves * kWaveSize) void draft_verify_pick(
 //   fp32         10.4/14.1   10.8/14.1  15.6/14.1  29.4/14.3       13.7/14.1  20.0/14.5        43.1/43.6
 //   fp64         10.6/14.2   14.4/14.2  24.0/14.1  55.8/14.3       20.9/14.6  35.7/17.3        79.5/73.4
 // Between the columns of 32768 and 65536 the two cross for one sequence; fp64, which has half the packets' classes,
-// loses above 16384 with several. Beyond two sequences per compute unit neither side is ahead by more than a sixth, and
+// loses above 16384 with several. Beyond two sequences per compute unit neither side is ahead by more than a fifth, and
 // whole rows need no scratch. Rows are cut into parts of 4 to 64 runs per wavefront, as many as 16
 // workgroups per compute unit make of them: short streams, of neighbouring workgroups, lie close
 // together in memory (fp32 [192, 6, 131072]: 47 us with 5 workgroups per compute unit, 38 with 16,
